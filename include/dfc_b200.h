@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define DFC_ABI_VERSION 3
+#define DFC_ABI_VERSION 4
 
 /* Entry points are the library's only exported symbols (it is built with
  * -fvisibility=hidden). */
@@ -54,6 +54,7 @@ extern "C" {
 #define DFC_ERR_CUDA (-7)      /* CUDA runtime error (see dfc_last_cuda_error) */
 #define DFC_ERR_RANGE (-8)     /* bit range outside the fiber */
 #define DFC_ERR_SCRATCH (-9)   /* scratch buffer too small */
+#define DFC_ERR_VALUE (-10)    /* scalar argument outside its range */
 
 /* ---- moment-word formats ---- */
 /* FP32 moments, second moment used as stored (enable_fiber=False,
@@ -165,6 +166,27 @@ typedef struct DfcWordRange {
   uint32_t* words;
   int64_t count;
 } DfcWordRange;
+
+/* Dropout of one call (no reference counterpart).  Element i of the output,
+ * counted in row-major order, is kept when its 32-bit word u_i is at least
+ * floor(p * 2^32 + 1/2); u_i comes from Philox4x32-10 with key `seed` and
+ * counter (i / 8, offset): one Philox block holds the high 16 bits of eight
+ * elements' words, the block with the top bit of the counter's second word
+ * set holds their low 16 bits.  state: NULL, or two uint64 in device memory,
+ * read when the kernel runs: the seed is then state[0] and the offset
+ * state[1] + offset (modulo 2^64), so a captured graph draws new masks when
+ * the words change between replays.  p in [0, 1].  32 bytes. */
+typedef struct DfcDropout {
+  uint64_t seed;
+  uint64_t offset;
+  const uint64_t* state;
+  double p;
+} DfcDropout;
+
+/* Limits of the token-table calls. */
+#define DFC_MAX_TOKENS (INT64_C(1) << 28)
+#define DFC_MAX_VOCAB (INT64_C(1) << 30)
+#define DFC_MAX_DIM (INT64_C(1) << 20)
 
 DFC_API int dfc_abi_version(void);
 DFC_API const char* dfc_strerror(int status);
@@ -380,6 +402,56 @@ DFC_API int dfc_multicast_sum_bf16(const void* comp_multicast, float* out, int64
 DFC_API int dfc_peer_barrier(uint32_t* const* slot_ptrs, int32_t n_peers, int32_t rank,
                              uint32_t epoch, int32_t* error_flag, int64_t timeout_ns,
                              void* stream);
+
+/*
+ * Dropout with a mask that is computed, never stored (no reference
+ * counterpart): y = residual + (kept ? x / (1 - p) : 0) over n elements of
+ * one type, computed in FP32 and rounded once.  A dropped element is zero
+ * whatever x holds.  residual may be NULL.  y may be x or residual itself;
+ * otherwise the buffers must not overlap.  The gradient with respect to x is
+ * the same call on dy without a residual.  dropout == NULL: nothing dropped.
+ * n <= 2^39.
+ */
+DFC_API int dfc_dropout(const void* x, const void* residual, void* y, int64_t n, int32_t dtype,
+                        const DfcDropout* dropout, void* stream);
+
+/*
+ * Rows of a token table (no reference counterpart): out[t] = drop(scale *
+ * table[tokens[t]]) for t < n_tokens, in FP32, rounded once to out_dtype; out
+ * is contiguous (n_tokens x dim) and dropout counts its elements.
+ * token_bytes: 4 (int32) or 8 (int64).  table: vocab rows of dim elements,
+ * table_pitch elements apart.  A token outside [0, vocab) reads nothing: its
+ * row is NaN where dropout keeps it, and *error_flag (an int that the device
+ * can write, or NULL) is set to 1.  dropout may be NULL.
+ */
+DFC_API int dfc_embedding(const void* tokens, int32_t token_bytes, int64_t n_tokens,
+                          const void* table, int32_t table_dtype, int64_t table_pitch,
+                          int64_t vocab, int64_t dim, float scale, void* out, int32_t out_dtype,
+                          const DfcDropout* dropout, int32_t* error_flag, void* stream);
+
+/*
+ * The table's gradient (no reference counterpart): the tokens are sorted
+ * (stable) and each run of equal tokens is summed, so
+ * grad[v] (+)= scale * sum over t with tokens[t] = v of drop(dy[t]), summed in
+ * FP32 in an order that depends on the tokens, n_tokens, dim and the types
+ * alone (the same inputs give the same bits), rounded once to grad_dtype.
+ * dropout is the lookup's (its element t * dim + d).
+ * dy: n_tokens rows, dy_pitch elements apart; grad: vocab rows, grad_pitch
+ * >= dim elements apart.  accumulate != 0: added to grad, rows without a token
+ * are not touched; 0: grad is overwritten, rows without a token become zero.
+ * Tokens equal to padding_idx (pass -1 for none) contribute nothing, nor do
+ * tokens outside [0, vocab), which set *error_flag (or NULL) to 1.
+ * scratch (device, 16-byte aligned) holds at least
+ * dfc_embedding_grad_scratch_bytes() bytes and is free again once the call's
+ * work on the stream is done.
+ */
+DFC_API size_t dfc_embedding_grad_scratch_bytes(int64_t n_tokens, int64_t vocab, int64_t dim);
+DFC_API int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64_t n_tokens,
+                               const void* dy, int32_t dy_dtype, int64_t dy_pitch, void* grad,
+                               int32_t grad_dtype, int64_t grad_pitch, int64_t vocab, int64_t dim,
+                               float scale, int64_t padding_idx, int32_t accumulate,
+                               const DfcDropout* dropout, int32_t* error_flag, void* scratch,
+                               size_t scratch_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,7 @@ from . import build as _build
 LIB_PATH = _build.LIB_PATH
 
 # ---- status codes / enums (mirror include/dfc_b200.h) ----
-ABI_VERSION = 3
+ABI_VERSION = 4
 DFC_OK = 0
 DFC_ERR_NULL = -1
 DFC_ERR_ALIGN = -2
@@ -29,6 +29,7 @@ DFC_ERR_HYPER = -6
 DFC_ERR_CUDA = -7
 DFC_ERR_RANGE = -8
 DFC_ERR_SCRATCH = -9
+DFC_ERR_VALUE = -10
 
 # partial records available to dfc_grad_stats_noalloc (include/dfc_b200.h)
 GRAD_STATS_STATIC_RECORDS = 65536
@@ -63,12 +64,13 @@ PEERSEG_DTYPE = np.dtype([("offset", "<i8"), ("numel", "<i8"), ("exp_avg", "<u8"
                           ("exp_avg_sq", "<u8"), ("hyper", "<i4"), ("reserved", "<i4")])
 COMPRESSRANGE_DTYPE = np.dtype([("grad", "<u8"), ("comp", "<u8"), ("resid", "<u8"),
                                 ("numel", "<i8")])
+DROPOUT_DTYPE = np.dtype([("seed", "<u8"), ("offset", "<u8"), ("state", "<u8"), ("p", "<f8")])
 MAX_PEERS = 8
 FUSED_AFTER_BARRIER = 1  # dfc_zero_fused_step_ef flag
 assert SEGMENT_DTYPE.itemsize == 48 and HYPER_DTYPE.itemsize == 48
 assert GRADREF_DTYPE.itemsize == 24 and GRADSTATS_DTYPE.itemsize == 24
 assert WORDRANGE_DTYPE.itemsize == 16 and PEERSEG_DTYPE.itemsize == 40
-assert COMPRESSRANGE_DTYPE.itemsize == 32
+assert COMPRESSRANGE_DTYPE.itemsize == 32 and DROPOUT_DTYPE.itemsize == 32
 
 # Names of every entry point the header declares (checked by the CPU tests).
 EXPORTS = (
@@ -79,6 +81,7 @@ EXPORTS = (
     "dfc_zero_fused_step", "dfc_zero_fused_step_ef", "dfc_peer_barrier",
     "dfc_multicast_sum_bf16",
     "dfc_replay_encode", "dfc_replay_decode",
+    "dfc_dropout", "dfc_embedding", "dfc_embedding_grad_scratch_bytes", "dfc_embedding_grad",
 )
 
 
@@ -120,6 +123,12 @@ def _declare(h: ctypes.CDLL) -> None:
         "dfc_multicast_sum_bf16": ([P, P, I64, P], ctypes.c_int),
         "dfc_replay_encode": ([P, I64, P, P, I64, P, I64, P], ctypes.c_int),
         "dfc_replay_decode": ([P, I64, I64, P, P, P, P, P], ctypes.c_int),
+        "dfc_dropout": ([P, P, P, I64, I32, P, P], ctypes.c_int),
+        "dfc_embedding": ([P, I32, I64, P, I32, I64, I64, I64, ctypes.c_float, P, I32, P, P, P],
+                          ctypes.c_int),
+        "dfc_embedding_grad_scratch_bytes": ([I64, I64, I64], SZ),
+        "dfc_embedding_grad": ([P, I32, I64, P, I32, I64, P, I32, I64, I64, I64, ctypes.c_float,
+                                I64, I32, P, P, P, SZ, P], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(h, name)

@@ -48,6 +48,7 @@ extern "C" const char* dfc_strerror(int status) {
     case DFC_ERR_CUDA: return "CUDA runtime error";
     case DFC_ERR_RANGE: return "fiber range out of bounds";
     case DFC_ERR_SCRATCH: return "scratch buffer too small";
+    case DFC_ERR_VALUE: return "scalar argument outside its range";
     default: return "unknown status";
   }
 }
