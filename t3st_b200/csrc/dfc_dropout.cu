@@ -3,36 +3,42 @@
 // the element type.  The same call on dy with the same counter is the
 // gradient.  Dropped elements are zero whatever x holds (Inf and NaN too).
 //
-// One thread per group of eight elements: one Philox call and one 16-byte
-// access per 16-bit operand.  One CTA per tile of 2 x kThreads groups, in
-// address order (the shape dfc_compress_ef measured best), both groups' loads
-// issued before either is used.
+// One thread takes kGroups groups of eight elements: one Philox call and one
+// 16-byte access per 16-bit operand and group.  One CTA per tile of consecutive
+// groups, in address order (the shape dfc_compress_ef measured best), all
+// loads issued before the first is used.
 #include "dfc_philox.cuh"
 
 namespace dfc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = 2;  // groups per thread
+constexpr int kGroups = 4;  // groups per thread
 
+// Element accesses of group g, for any alignment and for a last group of
+// fewer than eight elements.
 template <typename T, bool RES, bool DROP>
-__device__ __forceinline__ void finish8(float (&v)[8], const Raw8<T>& r, uint64_t g,
-                                        const DropArgs& a, const DropKey& k) {
-  if (DROP) drop8(v, g, a, k);
-  if (RES) {
-    float f[8];
-    unpack8<T>(r, f);
+__device__ __forceinline__ void drop_group(const T* x, const T* res, T* y, int64_t g, int64_t n,
+                                           const DropArgs& a, const DropKey& k) {
+  uint4 w[1] = {};
+  if (DROP) drop_words<1>({static_cast<uint64_t>(g)}, a, k, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(f[j], v[j]);
+  for (int j = 0; j < 8; ++j) {
+    const int64_t i = 8 * g + j;
+    if (i < n) {
+      float v = to_f32(x[i]);
+      if (DROP) v = kept(w[0], j, a.cmp) ? __fmul_rn(v, a.scale) : 0.0f;
+      if (RES) v = __fadd_rn(to_f32(res[i]), v);
+      y[i] = from_f32<T>(v);
+    }
   }
 }
 
-// Groups of eight that lie on 16-byte boundaries.
+// x, res and y on 16-byte boundaries.
 template <typename T, bool RES, bool DROP>
 __global__ void __launch_bounds__(kThreads)
-    dropout_vec_kernel(const T* x, const T* res, T* y, int64_t groups, DropArgs a) {
-  DropKey k{};
-  if (DROP) k = drop_key(a);
+    dropout_vec_kernel(const T* x, const T* res, T* y, int64_t n, DropArgs a) {
+  const int64_t groups = n / 8;
   const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kGroups) + threadIdx.x;
   Raw8<T> X[kGroups], R[kGroups];
 #pragma unroll
@@ -43,39 +49,41 @@ __global__ void __launch_bounds__(kThreads)
       if (RES) R[u] = load8(res + 8 * g);
     }
   }
+  DropKey k{};
+  uint4 w[kGroups];
+  if (DROP) {
+    k = drop_key(a);
+    uint64_t g[kGroups];
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) g[u] = g0 + u * kThreads;
+    drop_words<kGroups>(g, a, k, w);
+  }
 #pragma unroll
   for (int u = 0; u < kGroups; ++u) {
     const int64_t g = g0 + u * kThreads;
     if (g < groups) {
       float v[8];
       unpack8<T>(X[u], v);
-      finish8<T, RES, DROP>(v, R[u], g, a, k);
+      if (DROP) drop8(v, w[u], a);
+      if (RES) {
+        float f[8];
+        unpack8<T>(R[u], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(f[j], v[j]);
+      }
       store8(y + 8 * g, pack8<T>(v));
+    } else if (g == groups && 8 * g < n) {
+      drop_group<T, RES, DROP>(x, res, y, g, n, a, k);
     }
   }
 }
 
-// Any alignment, and the last group when n is no multiple of eight: element
-// accesses, groups from first_group on.
 template <typename T, bool RES, bool DROP>
 __global__ void __launch_bounds__(kThreads)
-    dropout_any_kernel(const T* x, const T* res, T* y, int64_t first_group, int64_t n, DropArgs a) {
+    dropout_any_kernel(const T* x, const T* res, T* y, int64_t n, DropArgs a) {
   DropKey k{};
   if (DROP) k = drop_key(a);
-  const int64_t g = first_group + static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (8 * g >= n) return;
-  uint4 w{};
-  if (DROP) w = drop_words(g, a, k);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int64_t i = 8 * g + j;
-    if (i < n) {
-      float v = to_f32(x[i]);
-      if (DROP) v = kept(w, j, a.cmp) ? __fmul_rn(v, a.scale) : 0.0f;
-      if (RES) v = __fadd_rn(to_f32(res[i]), v);
-      y[i] = from_f32<T>(v);
-    }
-  }
+  drop_group<T, RES, DROP>(x, res, y, static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, n, a, k);
 }
 
 template <typename T, bool RES, bool DROP>
@@ -83,19 +91,14 @@ int launch(const void* x, const void* res, void* y, int64_t n, const DropArgs& a
   const T* px = static_cast<const T*>(x);
   const T* pr = static_cast<const T*>(res);
   T* py = static_cast<T*>(y);
-  int64_t done = 0;
-  if (aligned(x, 16) && aligned(res, 16) && aligned(y, 16)) {
-    done = n / 8;
-    const int64_t tile = kThreads * kGroups;
-    if (done > 0)
-      dropout_vec_kernel<T, RES, DROP>
-          <<<static_cast<unsigned>((done + tile - 1) / tile), kThreads, 0, st>>>(px, pr, py, done, a);
-  }
-  const int64_t rest = (n + 7) / 8 - done;
-  if (rest > 0)
-    dropout_any_kernel<T, RES, DROP>
-        <<<static_cast<unsigned>((rest + kThreads - 1) / kThreads), kThreads, 0, st>>>(px, pr, py,
-                                                                                     done, n, a);
+  const int64_t groups = (n + 7) / 8;
+  const bool vec = aligned(x, 16) && aligned(res, 16) && aligned(y, 16);
+  const int64_t tile = vec ? kThreads * kGroups : kThreads;
+  const unsigned grid = static_cast<unsigned>((groups + tile - 1) / tile);
+  if (vec)
+    dropout_vec_kernel<T, RES, DROP><<<grid, kThreads, 0, st>>>(px, pr, py, n, a);
+  else
+    dropout_any_kernel<T, RES, DROP><<<grid, kThreads, 0, st>>>(px, pr, py, n, a);
   return launch_status();
 }
 

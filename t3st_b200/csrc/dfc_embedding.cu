@@ -13,7 +13,7 @@ namespace dfc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = 2;
+constexpr int kGroups = 4;  // groups per thread
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_t t) {
   return wide ? static_cast<const int64_t*>(tokens)[t]
@@ -25,8 +25,6 @@ __global__ void __launch_bounds__(kThreads)
     embed_vec_kernel(const void* tokens, int wide, const TT* table, int64_t pitch, int64_t vocab,
                      uint32_t row_groups, int64_t groups, float scale, TO* out, int32_t* error_flag,
                      DropArgs a) {
-  DropKey k{};
-  if (DROP) k = drop_key(a);
   const int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads * kGroups);
   const int64_t t0 = base / row_groups;
   const uint32_t c0 = static_cast<uint32_t>(base - t0 * row_groups);
@@ -43,6 +41,13 @@ __global__ void __launch_bounds__(kThreads)
       if (!bad[u]) X[u] = load8(table + v * pitch + 8ll * (q - dt * row_groups));
     }
   }
+  uint4 w[kGroups];
+  if (DROP) {
+    uint64_t g[kGroups];
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) g[u] = base + u * kThreads + threadIdx.x;
+    drop_words<kGroups>(g, a, drop_key(a), w);
+  }
 #pragma unroll
   for (int u = 0; u < kGroups; ++u) {
     const int64_t g = base + u * kThreads + threadIdx.x;
@@ -57,7 +62,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], scale);
       }
-      if (DROP) drop8(v, g, a, k);
+      if (DROP) drop8(v, w[u], a);
       store8(out + 8 * g, pack8<TO>(v));
     }
   }
@@ -68,8 +73,6 @@ __global__ void __launch_bounds__(kThreads)
     embed_any_kernel(const void* tokens, int wide, const TT* table, int64_t pitch, int64_t vocab,
                      int64_t dim, int64_t n, float scale, TO* out, int out_aligned,
                      int32_t* error_flag, DropArgs a) {
-  DropKey k{};
-  if (DROP) k = drop_key(a);
   const int64_t g = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (8 * g >= n) return;
   int64_t t = 8 * g / dim;
@@ -93,7 +96,11 @@ __global__ void __launch_bounds__(kThreads)
       ++d;
     }
   }
-  if (DROP) drop8(x, g, a, k);
+  if (DROP) {
+    uint4 w[1];
+    drop_words<1>({static_cast<uint64_t>(g)}, a, drop_key(a), w);
+    drop8(x, w[0], a);
+  }
   if (out_aligned && 8 * g + 8 <= n) {
     store8(out + 8 * g, pack8<TO>(x));
   } else {

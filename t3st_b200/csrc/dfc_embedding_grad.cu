@@ -2,14 +2,17 @@
 // grad[v] (+)= scale * sum over t with tokens[t] = v, t ascending, of drop(dy[t]).
 //
 //   1. a stable radix sort of (token, position) pairs; padding and
-//      out-of-range tokens get the key `vocab` and sort behind the others;
+//      out-of-range tokens get the key `vocab` and sort behind the others.  Up
+//      to 131,072 tokens one cluster of CTAs sorts in its shared memory;
 //   2. sum_kernel: the sorted positions are cut into tiles of K; one thread
 //      holds eight columns of a tile and adds its rows in order in FP32
 //      registers, writing a row of grad at each end of a run.  A run that
-//      crosses tile borders leaves FP32 partial rows in the scratch instead;
-//   3. join_kernel adds such a run's partial rows in a fixed order;
-//   4. fill_kernel zeroes the rows of an overwritten grad that no token names.
+//      crosses tile borders leaves FP32 partial rows in the scratch instead.
+//      The same grid zeroes the rows of an overwritten grad that no token names;
+//   3. join_kernel adds such a run's partial rows in a fixed order.
 // No atomics on floats: the same inputs give the same bits.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "dfc_philox.cuh"
@@ -17,7 +20,16 @@
 namespace dfc {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr uint32_t kNoKey = 0xFFFFFFFFu;
+
+// Programmatic dependent launch: the next kernel's CTAs may become resident
+// early; they wait here until the kernel before is complete.
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- 1. sort ------------------------------------------------------------------
 constexpr int kSortThreads = 256;
@@ -33,6 +45,7 @@ struct Tokens {
   int64_t vocab;
   int64_t padding_idx;
   int32_t* error_flag;
+  uint8_t* named;        // NULL, or one byte per row: a token names it
 };
 
 __device__ __forceinline__ uint32_t token_key(const Tokens& tk, int64_t t) {
@@ -151,6 +164,129 @@ __global__ void __launch_bounds__(kSortThreads)
       const uint32_t at = count[warp][(key[r] >> shift) & (bins - 1)] + rank[r];
       out_keys[at] = key[r];
       out_pos[at] = keys ? pos[i] : static_cast<uint32_t>(i);
+      if (!keys && tk.named && key[r] < tk.vocab) tk.named[key[r]] = 1;
+    }
+  }
+}
+
+// The whole sort in one cluster: CTA q holds the items [q * chunk, (q + 1) *
+// chunk) of the current order in registers, ITEMS a thread.  A pass counts
+// the digits of each warp's items, turns the counts into places (prefix over
+// the warps here, over the digits and CTAs through distributed shared memory)
+// and sends each item to the CTA that owns its place; the last pass writes to
+// global memory.
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kMaxClusterItems = 16;
+// rows whose `named` bytes the cluster clears itself
+constexpr int64_t kClusterClears = 1 << 20;
+
+template <int ITEMS>
+constexpr size_t cluster_smem(int bins) {
+  return static_cast<size_t>(bins) * (2 * kClusterWarps + 4 + 4) + 8 * kClusterThreads * ITEMS;
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kClusterThreads, 1)
+    sort_cluster_kernel(Tokens tk, int64_t n, int passes, int digit_bits, uint32_t* out_keys,
+                        uint32_t* out_pos) {
+  constexpr uint32_t kChunk = kClusterThreads * ITEMS;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint32_t warp_sum[kClusterWarps];
+  const int bins = 1 << digit_bits;
+  uint2* buffer = reinterpret_cast<uint2*>(smem);
+  uint32_t* total = reinterpret_cast<uint32_t*>(smem + 8 * kChunk);
+  uint32_t* base = total + bins;
+  uint16_t* count = reinterpret_cast<uint16_t*>(base + bins);  // [warp][bin]
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t item0 = warp * (ITEMS * 32) + lane;  // + 32 per round
+  uint32_t key[ITEMS], pos[ITEMS];
+  let_next_start();
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    pos[r] = rank * kChunk + item0 + 32 * r;
+    key[r] = pos[r] < n ? token_key(tk, pos[r]) : 0u;
+  }
+  if (tk.named && tk.vocab <= kClusterClears) {
+    const uint32_t words = static_cast<uint32_t>((tk.vocab + 15) / 16);
+    for (uint32_t i = rank * kClusterThreads + threadIdx.x; i < words; i += ctas * kClusterThreads)
+      reinterpret_cast<uint4*>(tk.named)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * digit_bits;
+    for (int i = threadIdx.x; i < bins * kClusterWarps / 2; i += kClusterThreads)
+      reinterpret_cast<uint32_t*>(count)[i] = 0u;
+    __syncthreads();
+    uint16_t* mine = count + warp * bins;
+    uint32_t place[ITEMS];
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      const bool on = rank * kChunk + item0 + 32 * r < n;
+      const uint32_t d = on ? (key[r] >> shift) & (bins - 1) : kNoKey;
+      const uint32_t same = __match_any_sync(0xFFFFFFFFu, d);
+      const uint32_t before = on ? mine[d] : 0u;
+      place[r] = before + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (on && (same >> lane) == 1u) mine[d] = static_cast<uint16_t>(place[r] + 1);
+      __syncwarp();
+    }
+    __syncthreads();
+    if (threadIdx.x < bins) {
+      uint32_t run = 0;
+#pragma unroll 8
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const uint32_t c = count[w * bins + threadIdx.x];
+        count[w * bins + threadIdx.x] = static_cast<uint16_t>(run);
+        run += c;
+      }
+      total[threadIdx.x] = run;
+    }
+    cluster.sync();
+    uint32_t all = 0, earlier = 0, inc = 0;
+    if (threadIdx.x < bins) {
+      for (uint32_t q = 0; q < ctas; ++q) {
+        const uint32_t c = cluster.map_shared_rank(total, q)[threadIdx.x];
+        if (q < rank) earlier += c;
+        all += c;
+      }
+    }
+    inc = warp_inclusive(all);
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    if (warp == 0) warp_sum[lane] = warp_inclusive(warp_sum[lane]);
+    __syncthreads();
+    if (threadIdx.x < bins)
+      base[threadIdx.x] = earlier + inc - all + (warp > 0 ? warp_sum[warp - 1] : 0u);
+    __syncthreads();
+    const bool last = p + 1 == passes;
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+      if (rank * kChunk + item0 + 32 * r < n) {
+        const uint32_t d = (key[r] >> shift) & (bins - 1);
+        const uint32_t at = base[d] + mine[d] + place[r];
+        if (last) {
+          out_keys[at] = key[r];
+          out_pos[at] = pos[r];
+        } else {
+          cluster.map_shared_rank(buffer, at / kChunk)[at % kChunk] = make_uint2(key[r], pos[r]);
+        }
+        // the bytes were cleared before the barrier of the first pass
+        if (p == 0 && tk.named && key[r] < tk.vocab) tk.named[key[r]] = 1;
+      }
+    }
+    cluster.sync();  // the items have arrived; no CTA leaves while others read its counts
+    if (!last) {
+#pragma unroll
+      for (int r = 0; r < ITEMS; ++r) {
+        if (rank * kChunk + item0 + 32 * r < n) {
+          const uint2 kp = buffer[item0 + 32 * r];
+          key[r] = kp.x;
+          pos[r] = kp.y;
+        }
+      }
     }
   }
 }
@@ -170,36 +306,50 @@ struct SumArgs {
   int accumulate;
   float* partial;        // 2 rows a tile: a run from before it, a run that goes on behind it
   int64_t partial_pitch; // dim rounded up to 8
+  const uint8_t* named;  // one byte per row of an overwritten grad
   DropArgs drop;
 };
 
-// Columns c .. c + 7 (those below dim) of a row in FP32.
+// Columns c .. c + 7 (those below dim) of a row, from `at`, in FP32.
 template <typename T, bool VEC>
-__device__ __forceinline__ void row8(const T* row, int64_t c, int64_t dim, float (&v)[8]) {
+__device__ __forceinline__ void row8(const T* at, int64_t c, int64_t dim, float (&v)[8]) {
   if constexpr (VEC) {
-    unpack8<T>(load8(row + c), v);
+    unpack8<T>(load8(at), v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < dim ? to_f32(row[c + j]) : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = c + j < dim ? to_f32(at[j]) : 0.0f;
   }
 }
 
-// v[j] = element e + j kept ? v[j] : 0 (the scale is applied to the sum).
-template <bool VEC>
-__device__ __forceinline__ void mask8(float (&v)[8], int64_t e, const DropArgs& a, const DropKey& k) {
-  const uint4 w = drop_words(e >> 3, a, k);
-  if (VEC || (e & 7) == 0) {
+// v[u][j] = element e[u] + j kept ? v[u][j] : 0 (the scale is applied to the sum).
+template <int N, bool VEC>
+__device__ __forceinline__ void mask8(float (&v)[N][8], const int64_t (&e)[N], const DropArgs& a,
+                                      const DropKey& k) {
+  uint64_t g[N];
+  uint4 w[N];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = kept(w, j, a.cmp) ? v[j] : 0.0f;
+  for (int u = 0; u < N; ++u) g[u] = static_cast<uint64_t>(e[u]) >> 3;
+  drop_words<N>(g, a, k, w);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[u][j] = kept(w[u], j, a.cmp) ? v[u][j] : 0.0f;
   } else {
-    const uint4 x = drop_words((e >> 3) + 1, a, k);
-    uint32_t bits = 0;
+    uint4 x[N];  // the eight elements reach into the next group
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      bits |= (kept(w, j, a.cmp) ? 1u << j : 0u) | (kept(x, j, a.cmp) ? 256u << j : 0u);
-    bits >>= e & 7;
+    for (int u = 0; u < N; ++u) ++g[u];
+    drop_words<N>(g, a, k, x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.0f;
+    for (int u = 0; u < N; ++u) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        bits |= (kept(w[u], j, a.cmp) ? 1u << j : 0u) | (kept(x[u], j, a.cmp) ? 256u << j : 0u);
+      bits >>= e[u] & 7;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[u][j] = (bits >> j) & 1u ? v[u][j] : 0.0f;
+    }
   }
 }
 
@@ -210,7 +360,7 @@ __device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t
   for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], s.scale);
   if (s.accumulate) {
     float g[8];
-    row8<TG, VEC>(row, c, s.dim, g);
+    row8<TG, VEC>(row + c, c, s.dim, g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(g[j], v[j]);
   }
@@ -224,40 +374,71 @@ __device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t
 }
 
 constexpr int kSumThreads = 128;
+constexpr int kSumLanes = 64;  // threads of a tile's slab of 512 columns, at most
 constexpr int kBatch = 4;
+constexpr int kFillRows = 32;
 
+// Zeros for the rows [first, first + rows) that no token names.
+template <typename TG, bool VEC>
+__device__ __forceinline__ void fill(const SumArgs& s, int64_t first, int rows) {
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid & 31;
+  const int64_t mine = first + lane;
+  const uint32_t empty = __ballot_sync(0xFFFFFFFFu, lane < rows && mine < s.vocab && !s.named[mine]);
+  for (int r = 0; r < rows; ++r) {
+    if (!((empty >> r) & 1u)) continue;
+    TG* row = static_cast<TG*>(s.grad) + (first + r) * s.grad_pitch;
+    if constexpr (VEC) {
+      const float z[8] = {};
+      for (int64_t c = 8ll * tid; c < s.dim; c += 8 * kSumThreads) store8(row + c, pack8<TG>(z));
+    } else {
+      for (int64_t c = tid; c < s.dim; c += kSumThreads) row[c] = from_f32<TG>(0.0f);
+    }
+  }
+}
+
+// CTAs [0, sum_ctas): blockDim.y units, each a slab of 8 * blockDim.x columns
+// of a tile.  CTAs behind them: fill_rows rows each.
 template <typename TD, typename TG, bool DROP, bool VEC>
-__global__ void __launch_bounds__(kSumThreads) sum_kernel(SumArgs s) {
-  const int64_t c = 8 * (static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x);
-  const int64_t tile = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+__global__ void __launch_bounds__(kSumThreads) sum_kernel(SumArgs s, uint32_t slabs, uint32_t sum_ctas,
+                                                          int fill_rows) {
+  let_next_start();
+  wait_for_previous();
+  if (blockIdx.x >= sum_ctas) {
+    fill<TG, VEC>(s, static_cast<int64_t>(blockIdx.x - sum_ctas) * fill_rows, fill_rows);
+    return;
+  }
+  const uint32_t unit = blockIdx.x * blockDim.y + threadIdx.y;
+  const int64_t tile = unit / slabs;
+  const int64_t c = 8ll * ((unit % slabs) * blockDim.x + threadIdx.x);
   const int64_t lo = tile * s.tile;
   if (c >= s.dim || lo >= s.n) return;
   const int64_t hi = min(lo + s.tile, s.n);
   DropKey k{};
   if (DROP) k = drop_key(s.drop);
-  const TD* dy = static_cast<const TD*>(s.dy);
+  const TD* dy = static_cast<const TD*>(s.dy) + c;
   const uint32_t before = lo > 0 ? s.keys[lo - 1] : kNoKey;
   const uint32_t behind = hi < s.n ? s.keys[hi] : kNoKey;
   float acc[8];
   uint32_t run = kNoKey;
   bool first = true;  // no row of the tile has ended a run yet
   for (int64_t i = lo; i < hi; i += kBatch) {
-    uint32_t key[kBatch];
+    // i is a multiple of kBatch, and the arrays are allocated in whole tiles
+    const uint4 k4 = *reinterpret_cast<const uint4*>(s.keys + i);
+    const uint4 p4 = *reinterpret_cast<const uint4*>(s.pos + i);
+    uint32_t key[kBatch] = {k4.x, k4.y, k4.z, k4.w};
+    const uint32_t p[kBatch] = {p4.x, p4.y, p4.z, p4.w};
     float v[kBatch][8];
-    int64_t p[kBatch];
+    int64_t e[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const bool on = i + u < hi;
-      key[u] = on ? s.keys[i + u] : kNoKey;
-      p[u] = on ? s.pos[i + u] : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
+      if (i + u >= hi) key[u] = kNoKey;
       if (key[u] < s.vocab) row8<TD, VEC>(dy + p[u] * s.dy_pitch, c, s.dim, v[u]);
+      e[u] = p[u] * s.dim + c;
+    }
+    if (DROP) mask8<kBatch, VEC>(v, e, s.drop, k);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       if (key[u] >= s.vocab) continue;
-      if (DROP) mask8<VEC>(v[u], p[u] * s.dim + c, s.drop, k);
       if (key[u] == run) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] = __fadd_rn(acc[j], v[u][j]);
@@ -285,52 +466,52 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(SumArgs s) {
 }
 
 // ---- 3. runs that cross tile borders --------------------------------------------
-constexpr int kJoinWarps = 8;
+constexpr int kJoinLanes = 64;
+constexpr int kJoinParts = 4;
+constexpr int kJoinThreads = kJoinLanes * kJoinParts;
 
-// Tile blockIdx.x, if a run begins in it and goes on behind it; columns 4 per
-// lane.  Warp w adds partial rows w, w + 8, ... of the run, warp 0 the eight sums.
+__device__ __forceinline__ void add4(float4& a, const float4& b) {
+  a.x = __fadd_rn(a.x, b.x);
+  a.y = __fadd_rn(a.y, b.y);
+  a.z = __fadd_rn(a.z, b.z);
+  a.w = __fadd_rn(a.w, b.w);
+}
+
+// Tile blockIdx.x, if a run begins in it and goes on behind it; 4 columns per
+// lane.  Part q adds the run's partial rows q, q + 4, ...; part 0 the four sums.
 template <typename TG>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(SumArgs s) {
-  __shared__ float4 sums[kJoinWarps][32];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(SumArgs s) {
+  __shared__ float4 sums[kJoinParts][kJoinLanes];
+  let_next_start();
+  wait_for_previous();
   const int64_t tile = blockIdx.x;
   const int64_t lo = tile * s.tile, hi = lo + s.tile;
   if (hi >= s.n) return;
-  const uint32_t key = s.keys[hi - 1];
-  if (key >= s.vocab || s.keys[hi] != key) return;
-  if (lo > 0 && s.keys[lo - 1] == key) return;  // it began earlier
-  // the last tile whose first item still has the key
-  int64_t last = tile + 1, end = (s.n - 1) / s.tile;
-  while (last < end) {
-    const int64_t mid = (last + end + 1) / 2;
-    if (s.keys[mid * s.tile] == key)
-      last = mid;
-    else
-      end = mid - 1;
+  const uint32_t key = s.keys[hi - 1], behind = s.keys[hi];
+  const uint32_t before = lo > 0 ? s.keys[lo - 1] : kNoKey;
+  if (key >= s.vocab || behind != key || before == key) return;
+  // the tiles behind this one whose first item has the key are consecutive
+  const int tid = threadIdx.y * kJoinLanes + threadIdx.x;
+  int64_t more = 0;
+  for (int found = kJoinThreads; found == kJoinThreads; more += found) {
+    const int64_t i = (tile + 1 + more + tid) * s.tile;
+    found = __syncthreads_count(i < s.n && s.keys[i] == key);
   }
-  const int64_t c = 4 * (static_cast<int64_t>(blockIdx.y) * 32 + threadIdx.x);
+  const int64_t c = 4 * (static_cast<int64_t>(blockIdx.y) * kJoinLanes + threadIdx.x);
   const bool on = c < s.dim;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (on) {
-    for (int64_t j = threadIdx.y; j <= last - tile; j += kJoinWarps) {
+#pragma unroll 4
+    for (int64_t j = threadIdx.y; j <= more; j += kJoinParts) {
       const int64_t row = j == 0 ? 2 * tile + 1 : 2 * (tile + j);
-      const float4 v = *reinterpret_cast<const float4*>(s.partial + row * s.partial_pitch + c);
-      acc.x = __fadd_rn(acc.x, v.x);
-      acc.y = __fadd_rn(acc.y, v.y);
-      acc.z = __fadd_rn(acc.z, v.z);
-      acc.w = __fadd_rn(acc.w, v.w);
+      add4(acc, *reinterpret_cast<const float4*>(s.partial + row * s.partial_pitch + c));
     }
   }
   sums[threadIdx.y][threadIdx.x] = acc;
   __syncthreads();
   if (threadIdx.y != 0 || !on) return;
 #pragma unroll
-  for (int w = 1; w < kJoinWarps; ++w) {
-    const float4 v = sums[w][threadIdx.x];
-    acc.x = __fadd_rn(acc.x, v.x);
-    acc.y = __fadd_rn(acc.y, v.y);
-    acc.z = __fadd_rn(acc.z, v.z);
-    acc.w = __fadd_rn(acc.w, v.w);
-  }
+  for (int q = 1; q < kJoinParts; ++q) add4(acc, sums[q][threadIdx.x]);
   const float f[4] = {acc.x, acc.y, acc.z, acc.w};
   TG* row = static_cast<TG*>(s.grad) + key * s.grad_pitch;
 #pragma unroll
@@ -343,47 +524,36 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(SumArgs s) {
   }
 }
 
-// ---- 4. rows without a token -----------------------------------------------------
-constexpr int kFillThreads = 256;
-constexpr int kFillRows = 32;
+// ---- host -------------------------------------------------------------------------
+// Threads of a slab and slabs of a row.
+struct Shape {
+  int lanes;
+  int64_t slabs;
+};
 
-template <typename TG, bool VEC>
-__global__ void __launch_bounds__(kFillThreads) fill_kernel(SumArgs s, int rows) {
-  __shared__ int empty[kFillRows];
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * rows;
-  if (threadIdx.x < rows) {
-    const int64_t v = first + threadIdx.x;
-    int64_t a = 0, b = s.n;  // the first sorted key >= v
-    while (a < b) {
-      const int64_t m = (a + b) / 2;
-      if (s.keys[m] < v)
-        a = m + 1;
-      else
-        b = m;
-    }
-    empty[threadIdx.x] = v < s.vocab && !(a < s.n && s.keys[a] == v);
-  }
-  __syncthreads();
-  for (int r = 0; r < rows; ++r) {
-    if (!empty[r]) continue;
-    TG* row = static_cast<TG*>(s.grad) + (first + r) * s.grad_pitch;
-    if constexpr (VEC) {
-      const float z[8] = {};
-      for (int64_t c = 8ll * threadIdx.x; c < s.dim; c += 8 * kFillThreads) store8(row + c, pack8<TG>(z));
-    } else {
-      for (int64_t c = threadIdx.x; c < s.dim; c += kFillThreads) row[c] = from_f32<TG>(0.0f);
-    }
-  }
+Shape shape(int64_t dim) {
+  const int64_t need = (dim + 7) / 8;
+  int lanes = 1;
+  while (lanes < need && lanes < kSumLanes) lanes *= 2;
+  return {lanes, (need + lanes - 1) / lanes};
 }
 
-// ---- host -------------------------------------------------------------------------
-int tile_tokens(int64_t, int64_t) { return 32; }
+// K: enough units for every SM, no more partial rows than that takes.
+constexpr int kMinTile = 8, kMaxTile = 256, kUnits = 2400;
+
+int tile_tokens(int64_t n, int64_t dim) {
+  const Shape sh = shape(dim);
+  const int64_t units_per_token = sh.slabs * sh.lanes;  // in threads
+  int tile = kMinTile;
+  while (tile < kMaxTile && tile * int64_t{kUnits} * kSumLanes < n * units_per_token) tile *= 2;
+  return tile;
+}
 
 struct Layout {
   int64_t sort_tiles;
   int passes, digit_bits, tile;
-  int64_t tiles, partial_pitch;
-  size_t keys[2], pos[2], hist, partial, bytes;
+  int64_t partial_pitch;
+  size_t keys[2], pos[2], hist, named, partial, bytes;
 };
 
 Layout layout(int64_t n, int64_t vocab, int64_t dim) {
@@ -394,7 +564,6 @@ Layout layout(int64_t n, int64_t vocab, int64_t dim) {
   l.digit_bits = (bits + l.passes - 1) / l.passes;
   l.sort_tiles = (n + kSortTile - 1) / kSortTile;
   l.tile = tile_tokens(n, dim);
-  l.tiles = (n + l.tile - 1) / l.tile;
   l.partial_pitch = (dim + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&at](int64_t bytes) {
@@ -402,14 +571,110 @@ Layout layout(int64_t n, int64_t vocab, int64_t dim) {
     at += static_cast<size_t>(bytes + 255) / 256 * 256;
     return here;
   };
-  for (int i = 0; i < 2; ++i) {
-    l.keys[i] = take(4 * n);
-    l.pos[i] = take(4 * n);
+  const int64_t whole = (n + kMaxTile - 1) / kMaxTile * kMaxTile;
+  const bool cluster = n <= int64_t{kMaxCluster} * kMaxClusterItems * kClusterThreads;
+  for (int i = 0; i < (cluster ? 1 : 2); ++i) {
+    l.keys[i] = take(4 * whole);
+    l.pos[i] = take(4 * whole);
   }
-  l.hist = take(l.sort_tiles * (int64_t{4} << l.digit_bits));
-  l.partial = take(8 * l.tiles * l.partial_pitch);
+  if (!cluster) l.hist = take(l.sort_tiles * (int64_t{4} << l.digit_bits));
+  l.named = take(vocab);
+  l.partial = take(8 * ((n + l.tile - 1) / l.tile) * l.partial_pitch);
   l.bytes = at;
   return l;
+}
+
+template <int ITEMS>
+cudaError_t sort_cluster(const Tokens& tk, int64_t n, int ctas, int passes, int digit_bits,
+                         uint32_t* keys, uint32_t* pos, cudaStream_t st) {
+  const size_t smem = cluster_smem<ITEMS>(1 << digit_bits);
+  if (smem > 40 * 1024) {  // with the static part, more than a kernel gets unasked
+    const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<ITEMS>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(cluster_smem<ITEMS>(kMaxBins)));
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sort_cluster_kernel<ITEMS>, tk, n, passes, digit_bits, keys, pos);
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch_next(Kernel kernel, dim3 grid, dim3 block, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+int failed(cudaError_t e) {
+  cudaGetLastError();
+  set_cuda_error(e);
+  return DFC_ERR_CUDA;
+}
+
+// Sorted keys and positions of the tokens (and tk.named): DFC_OK or an error.
+int sort_tokens(const Tokens& tk, int64_t n, const Layout& l, char* scratch, const uint32_t** keys_out,
+                const uint32_t** pos_out, cudaStream_t st) {
+  uint32_t *keys[2], *pos[2];
+  for (int i = 0; i < 2; ++i) {
+    keys[i] = reinterpret_cast<uint32_t*>(scratch + l.keys[i]);
+    pos[i] = reinterpret_cast<uint32_t*>(scratch + l.pos[i]);
+  }
+  *keys_out = keys[0];
+  *pos_out = pos[0];
+  const int64_t threads = (n + kClusterThreads - 1) / kClusterThreads;  // full CTAs at one item a thread
+  if (threads <= kMaxCluster * kMaxClusterItems) {
+    if (tk.named && tk.vocab > kClusterClears) {
+      const cudaError_t e = cudaMemsetAsync(tk.named, 0, static_cast<size_t>(tk.vocab), st);
+      if (e != cudaSuccess) return failed(e);
+    }
+    int ctas = 1, items = 1;
+    while (ctas < threads && ctas < kMaxCluster) ctas *= 2;
+    while (int64_t{ctas} * items < threads) items *= 2;
+    const auto sort = items == 1   ? sort_cluster<1>
+                      : items == 2 ? sort_cluster<2>
+                      : items == 4 ? sort_cluster<4>
+                      : items == 8 ? sort_cluster<8>
+                                   : sort_cluster<kMaxClusterItems>;
+    const cudaError_t e = sort(tk, n, ctas, l.passes, l.digit_bits, keys[0], pos[0], st);
+    return e == cudaSuccess ? DFC_OK : failed(e);
+  }
+  if (tk.named) {
+    const cudaError_t e = cudaMemsetAsync(tk.named, 0, static_cast<size_t>(tk.vocab), st);
+    if (e != cudaSuccess) return failed(e);
+  }
+  uint32_t* hist = reinterpret_cast<uint32_t*>(scratch + l.hist);
+  const unsigned tiles = static_cast<unsigned>(l.sort_tiles);
+  const int bins = 1 << l.digit_bits;
+  int from = 0;
+  for (int p = 0; p < l.passes; ++p) {
+    const uint32_t* k_in = p ? keys[from] : nullptr;
+    const int to = p ? 1 - from : 0;
+    sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(tk, k_in, n, p * l.digit_bits, bins, hist);
+    sort_scan_kernel<<<1, 1024, 0, st>>>(hist, l.sort_tiles * bins);
+    sort_scatter_kernel<<<tiles, kSortThreads, 0, st>>>(tk, k_in, pos[from], n, p * l.digit_bits, bins,
+                                                        hist, keys[to], pos[to]);
+    from = to;
+  }
+  *keys_out = keys[from];
+  *pos_out = pos[from];
+  return launch_status();
 }
 
 bool sizes_ok(int64_t n, int64_t vocab, int64_t dim) {
@@ -419,26 +684,23 @@ bool sizes_ok(int64_t n, int64_t vocab, int64_t dim) {
 
 template <typename TD, typename TG, bool DROP, bool VEC>
 int run_sums(const SumArgs& s, cudaStream_t st) {
+  const Shape sh = shape(s.dim);
   const int64_t tiles = (s.n + s.tile - 1) / s.tile;
-  const int64_t lanes_needed = (s.dim + 7) / 8;
-  int lanes = 1;
-  while (lanes < lanes_needed && lanes < kSumThreads) lanes *= 2;
-  const int subs = kSumThreads / lanes;
-  if (tiles > 0) {
-    const dim3 grid(static_cast<unsigned>((tiles + subs - 1) / subs),
-                    static_cast<unsigned>((lanes_needed + lanes - 1) / lanes));
-    sum_kernel<TD, TG, DROP, VEC><<<grid, dim3(lanes, subs), 0, st>>>(s);
-    if (tiles > 1) {
-      const dim3 jgrid(static_cast<unsigned>(tiles - 1), static_cast<unsigned>((s.dim + 127) / 128));
-      join_kernel<TG><<<jgrid, dim3(32, kJoinWarps), 0, st>>>(s);
-    }
-  }
-  if (!s.accumulate && s.vocab > 0) {
-    const int64_t row_bytes = s.dim * static_cast<int64_t>(sizeof(TG));
-    const int rows = static_cast<int>(std::min<int64_t>(kFillRows, std::max<int64_t>(1, 65536 / row_bytes)));
-    fill_kernel<TG, VEC><<<static_cast<unsigned>((s.vocab + rows - 1) / rows), kFillThreads, 0, st>>>(s, rows);
-  }
-  return launch_status();
+  const int subs = kSumThreads / sh.lanes;
+  const int64_t sum_ctas = (tiles * sh.slabs + subs - 1) / subs;
+  const int64_t row_bytes = s.dim * static_cast<int64_t>(sizeof(TG));
+  const int rows = static_cast<int>(std::min<int64_t>(kFillRows, std::max<int64_t>(1, 32768 / row_bytes)));
+  const int64_t fill_ctas = s.accumulate ? 0 : (s.vocab + rows - 1) / rows;
+  if (sum_ctas + fill_ctas == 0) return DFC_OK;
+  cudaError_t e = launch_next(sum_kernel<TD, TG, DROP, VEC>, dim3(static_cast<unsigned>(sum_ctas + fill_ctas)),
+                              dim3(sh.lanes, subs), st, s, static_cast<uint32_t>(sh.slabs),
+                              static_cast<uint32_t>(sum_ctas), rows);
+  if (e == cudaSuccess && tiles > 1)
+    e = launch_next(join_kernel<TG>,
+                    dim3(static_cast<unsigned>(tiles - 1),
+                         static_cast<unsigned>((s.dim + 4 * kJoinLanes - 1) / (4 * kJoinLanes))),
+                    dim3(kJoinLanes, kJoinParts), st, s);
+  return e == cudaSuccess ? launch_status() : failed(e);
 }
 
 template <typename TD, typename TG>
@@ -481,7 +743,7 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   const int rc = make_drop_args(dropout, &s.drop, &drop);
   if (rc != DFC_OK) return rc;
   if (dim == 0) return DFC_OK;
-  if ((!grad && vocab > 0) || (n_tokens > 0 && (!tokens || !dy || !scratch))) return DFC_ERR_NULL;
+  if ((!grad && vocab > 0) || !scratch || (n_tokens > 0 && (!tokens || !dy))) return DFC_ERR_NULL;
   if (!aligned(tokens, token_bytes) || !aligned(dy, dtype_size(dy_dtype)) ||
       !aligned(grad, dtype_size(grad_dtype)) || !aligned(error_flag, 4) || !aligned(scratch, 16))
     return DFC_ERR_ALIGN;
@@ -489,26 +751,16 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   if (scratch_bytes < l.bytes) return DFC_ERR_SCRATCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* base = static_cast<char*>(scratch);
-  uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(base + l.keys[0]), reinterpret_cast<uint32_t*>(base + l.keys[1])};
-  uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(base + l.pos[0]), reinterpret_cast<uint32_t*>(base + l.pos[1])};
-  uint32_t* hist = reinterpret_cast<uint32_t*>(base + l.hist);
-  const Tokens tk{tokens, token_bytes == 8, vocab, padding_idx, error_flag};
-  int from = 0;
+  uint8_t* named = accumulate ? nullptr : reinterpret_cast<uint8_t*>(base + l.named);
   if (n_tokens > 0) {
-    const unsigned tiles = static_cast<unsigned>(l.sort_tiles);
-    const int bins = 1 << l.digit_bits;
-    for (int p = 0; p < l.passes; ++p) {
-      const uint32_t* k_in = p ? keys[from] : nullptr;
-      const int to = p ? 1 - from : 0;
-      sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(tk, k_in, n_tokens, p * l.digit_bits, bins, hist);
-      sort_scan_kernel<<<1, 1024, 0, st>>>(hist, l.sort_tiles * bins);
-      sort_scatter_kernel<<<tiles, kSortThreads, 0, st>>>(tk, k_in, pos[from], n_tokens,
-                                                          p * l.digit_bits, bins, hist, keys[to], pos[to]);
-      from = to;
-    }
+    const Tokens tk{tokens, token_bytes == 8, vocab, padding_idx, error_flag, named};
+    const int rc = sort_tokens(tk, n_tokens, l, base, &s.keys, &s.pos, st);
+    if (rc != DFC_OK) return rc;
+  } else if (named && vocab > 0) {
+    const cudaError_t e = cudaMemsetAsync(named, 0, static_cast<size_t>(vocab), st);
+    if (e != cudaSuccess) return failed(e);
   }
-  s.keys = keys[from];
-  s.pos = pos[from];
+  s.named = named;
   s.n = n_tokens;
   s.tile = l.tile;
   s.dy = dy;

@@ -71,24 +71,27 @@ __device__ __forceinline__ DropKey drop_key(const DropArgs& a) {
           static_cast<uint32_t>(off), static_cast<uint32_t>(off >> 32)};
 }
 
+__device__ __forceinline__ void philox_round(uint32_t& c0, uint32_t& c1, uint32_t& c2, uint32_t& c3,
+                                             uint32_t k0, uint32_t k1) {
+  const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u;
+  const uint64_t b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
+  c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+  c1 = static_cast<uint32_t>(b);
+  c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+  c3 = static_cast<uint32_t>(a);
+}
+
 __device__ __forceinline__ uint4 philox10(uint32_t c0, uint32_t c1, const DropKey& k) {
   uint32_t c2 = k.o0, c3 = k.o1;
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u;
-    const uint64_t b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ (k.k0 + r * 0x9E3779B9u);
-    c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ (k.k1 + r * 0xBB67AE85u);
-    c3 = static_cast<uint32_t>(a);
-  }
+  for (int r = 0; r < 10; ++r)
+    philox_round(c0, c1, c2, c3, k.k0 + r * 0x9E3779B9u, k.k1 + r * 0xBB67AE85u);
   return make_uint4(c0, c1, c2, c3);
 }
 
-// Non-zero when a 16-bit half of w is zero.
-__device__ __forceinline__ uint32_t zero_half(uint32_t w) {
-  return (w - 0x00010001u) & ~w & 0x80008000u;
-}
+// Bit 15 or 31 is set when a 16-bit half of w is zero (and maybe when the
+// half below it is; never when neither is).
+__device__ __forceinline__ uint32_t zero_half(uint32_t w) { return (w - 0x00010001u) & ~w; }
 
 // A word of two high halves with its ties settled by the low halves.
 __device__ __forceinline__ uint32_t settle(uint32_t w, uint32_t low, const DropArgs& a) {
@@ -98,22 +101,56 @@ __device__ __forceinline__ uint32_t settle(uint32_t w, uint32_t low, const DropA
   return h0 | (h1 << 16);
 }
 
-// The comparison words of group g: kept(w, j) tells element j's fate.
-__device__ __forceinline__ uint4 drop_words(uint64_t g, const DropArgs& a, const DropKey& k) {
-  const uint32_t c0 = static_cast<uint32_t>(g), c1 = static_cast<uint32_t>(g >> 32);
-  uint4 w = philox10(c0, c1, k);
+// The comparison words of N groups: kept(w, j) tells element j's fate.  The
+// groups go through the rounds together: they share the round keys, and the
+// rare ties are looked for once.
+template <int N>
+__device__ __forceinline__ void drop_words(const uint64_t (&g)[N], const DropArgs& a, const DropKey& k,
+                                           uint4 (&w)[N]) {
+  uint32_t c0[N], c1[N], c2[N], c3[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    c0[i] = static_cast<uint32_t>(g[i]);
+    c1[i] = static_cast<uint32_t>(g[i] >> 32);
+    c2[i] = k.o0;
+    c3[i] = k.o1;
+  }
+  uint32_t k0 = k.k0, k1 = k.k1;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) philox_round(c0[i], c1[i], c2[i], c3[i], k0, k1);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = make_uint4(c0[i], c1[i], c2[i], c3[i]);
   if (a.t_lo) {
     const uint32_t t2 = a.t_hi * 0x00010001u;
-    if (zero_half(w.x ^ t2) | zero_half(w.y ^ t2) | zero_half(w.z ^ t2) | zero_half(w.w ^ t2)) {
-      const uint4 l = philox10(c0, c1 | 0x80000000u, k);
-      w.x = settle(w.x, l.x, a);
-      w.y = settle(w.y, l.y, a);
-      w.z = settle(w.z, l.z, a);
-      w.w = settle(w.w, l.w, a);
+    uint32_t tie = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      tie |= zero_half(w[i].x ^ t2) | zero_half(w[i].y ^ t2) | zero_half(w[i].z ^ t2) | zero_half(w[i].w ^ t2);
+    if (tie & 0x80008000u) {
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) {
+        const uint4 l = philox10(static_cast<uint32_t>(g[i]), static_cast<uint32_t>(g[i] >> 32) | 0x80000000u, k);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (i == j) {
+            w[j].x = settle(w[j].x, l.x, a);
+            w[j].y = settle(w[j].y, l.y, a);
+            w[j].z = settle(w[j].z, l.z, a);
+            w[j].w = settle(w[j].w, l.w, a);
+          }
+        }
+      }
     }
   }
-  if (a.all) w = make_uint4(0u, 0u, 0u, 0u);
-  return w;
+  if (a.all) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 
 __device__ __forceinline__ bool kept(const uint4& w, int j, uint32_t cmp) {
@@ -121,9 +158,8 @@ __device__ __forceinline__ bool kept(const uint4& w, int j, uint32_t cmp) {
   return ((j & 1) ? x : x << 16) >= cmp;
 }
 
-// Eight consecutive elements from group g: v[j] = kept ? v[j] * scale : 0.
-__device__ __forceinline__ void drop8(float (&v)[8], uint64_t g, const DropArgs& a, const DropKey& k) {
-  const uint4 w = drop_words(g, a, k);
+// Eight elements: v[j] = kept ? v[j] * scale : 0.
+__device__ __forceinline__ void drop8(float (&v)[8], const uint4& w, const DropArgs& a) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = kept(w, j, a.cmp) ? __fmul_rn(v[j], a.scale) : 0.0f;
 }
