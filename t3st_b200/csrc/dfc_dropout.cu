@@ -13,7 +13,13 @@ namespace dfc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = 4;  // groups per thread
+#ifndef DFC_DROP_GROUPS
+#define DFC_DROP_GROUPS 2
+#endif
+#ifndef DFC_DROP_BLOCKS
+#define DFC_DROP_BLOCKS 4
+#endif
+constexpr int kGroups = DFC_DROP_GROUPS;  // groups per thread
 
 // Element accesses of group g, for any alignment and for a last group of
 // fewer than eight elements.
@@ -36,8 +42,8 @@ __device__ __forceinline__ void drop_group(const T* x, const T* res, T* y, int64
 
 // x, res and y on 16-byte boundaries.
 template <typename T, bool RES, bool DROP>
-__global__ void __launch_bounds__(kThreads)
-    dropout_vec_kernel(const T* x, const T* res, T* y, int64_t n, DropArgs a) {
+__global__ void __launch_bounds__(kThreads, DFC_DROP_BLOCKS)
+    dropout_vec_kernel(const T* x, const T* res, T* y, int64_t n, int wide, DropArgs a) {
   const int64_t groups = n / 8;
   const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kGroups) + threadIdx.x;
   Raw8<T> X[kGroups], R[kGroups];
@@ -45,8 +51,8 @@ __global__ void __launch_bounds__(kThreads)
   for (int u = 0; u < kGroups; ++u) {
     const int64_t g = g0 + u * kThreads;
     if (g < groups) {
-      X[u] = load8(x + 8 * g);
-      if (RES) R[u] = load8(res + 8 * g);
+      X[u] = load8(x + 8 * g, wide);
+      if (RES) R[u] = load8(res + 8 * g, wide);
     }
   }
   DropKey k{};
@@ -71,7 +77,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(f[j], v[j]);
       }
-      store8(y + 8 * g, pack8<T>(v));
+      store8(y + 8 * g, pack8<T>(v), wide);
     } else if (g == groups && 8 * g < n) {
       drop_group<T, RES, DROP>(x, res, y, g, n, a, k);
     }
@@ -96,7 +102,8 @@ int launch(const void* x, const void* res, void* y, int64_t n, const DropArgs& a
   const int64_t tile = vec ? kThreads * kGroups : kThreads;
   const unsigned grid = static_cast<unsigned>((groups + tile - 1) / tile);
   if (vec)
-    dropout_vec_kernel<T, RES, DROP><<<grid, kThreads, 0, st>>>(px, pr, py, n, a);
+    dropout_vec_kernel<T, RES, DROP><<<grid, kThreads, 0, st>>>(
+        px, pr, py, n, aligned(x, 32) && aligned(res, 32) && aligned(y, 32), a);
   else
     dropout_any_kernel<T, RES, DROP><<<grid, kThreads, 0, st>>>(px, pr, py, n, a);
   return launch_status();

@@ -23,8 +23,8 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 template <typename TT, typename TO, bool DROP>
 __global__ void __launch_bounds__(kThreads)
     embed_vec_kernel(const void* tokens, int wide, const TT* table, int64_t pitch, int64_t vocab,
-                     uint32_t row_groups, int64_t groups, float scale, TO* out, int32_t* error_flag,
-                     DropArgs a) {
+                     uint32_t row_groups, int64_t groups, float scale, TO* out, int wide_table,
+                     int wide_out, int32_t* error_flag, DropArgs a) {
   const int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads * kGroups);
   const int64_t t0 = base / row_groups;
   const uint32_t c0 = static_cast<uint32_t>(base - t0 * row_groups);
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(kThreads)
       const uint32_t dt = q / row_groups;
       const int64_t v = token_at(tokens, wide, t0 + dt);
       bad[u] = static_cast<uint64_t>(v) >= static_cast<uint64_t>(vocab);
-      if (!bad[u]) X[u] = load8(table + v * pitch + 8ll * (q - dt * row_groups));
+      if (!bad[u]) X[u] = load8(table + v * pitch + 8ll * (q - dt * row_groups), wide_table);
     }
   }
   uint4 w[kGroups];
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], scale);
       }
       if (DROP) drop8(v, w[u], a);
-      store8(out + 8 * g, pack8<TO>(v));
+      store8(out + 8 * g, pack8<TO>(v), wide_out);
     }
   }
 }
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kThreads)
     drop8(x, w[0], a);
   }
   if (out_aligned && 8 * g + 8 <= n) {
-    store8(out + 8 * g, pack8<TO>(x));
+    store8(out + 8 * g, pack8<TO>(x), 0);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -134,7 +134,7 @@ int launch(const EmbedCall& c) {
     const int64_t groups = n / 8, tile = kThreads * kGroups;
     embed_vec_kernel<TT, TO, DROP><<<static_cast<unsigned>((groups + tile - 1) / tile), kThreads, 0, c.st>>>(
         c.tokens, c.wide, table, c.pitch, c.vocab, static_cast<uint32_t>(c.dim / 8), groups, c.scale,
-        out, c.error_flag, c.drop);
+        out, aligned(table, 32) && c.pitch % 8 == 0, aligned(out, 32), c.error_flag, c.drop);
   } else {
     const int64_t groups = (n + 7) / 8;
     embed_any_kernel<TT, TO, DROP>

@@ -232,21 +232,41 @@ __device__ __forceinline__ Raw8<T> pack8(const float (&v)[8]) {
   return r;
 }
 
-// 16-byte accesses; p is 16-byte aligned.
+// p is 16-byte aligned; FP32 with wide != 0: 32-byte aligned, and the eight
+// elements move in one access, so that a warp writes whole 32-byte sectors
+// (two 16-byte accesses 32 bytes apart write half sectors).
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T* p) {
+__device__ __forceinline__ Raw8<T> load8(const T* p, int wide) {
   Raw8<T> r;
   const uint4* q = reinterpret_cast<const uint4*>(p);
+  if constexpr (sizeof(T) == 4) {
+    if (wide) {
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r.q[0].x), "=r"(r.q[0].y), "=r"(r.q[0].z), "=r"(r.q[0].w), "=r"(r.q[1].x),
+                     "=r"(r.q[1].y), "=r"(r.q[1].z), "=r"(r.q[1].w)
+                   : "l"(p));
+      return r;
+    }
+    r.q[1] = q[1];
+  }
   r.q[0] = q[0];
-  if constexpr (sizeof(T) == 4) r.q[1] = q[1];
   return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const Raw8<T>& r) {
+__device__ __forceinline__ void store8(T* p, const Raw8<T>& r, int wide) {
   uint4* q = reinterpret_cast<uint4*>(p);
+  if constexpr (sizeof(T) == 4) {
+    if (wide) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r.q[0].x),
+                   "r"(r.q[0].y), "r"(r.q[0].z), "r"(r.q[0].w), "r"(r.q[1].x), "r"(r.q[1].y),
+                   "r"(r.q[1].z), "r"(r.q[1].w)
+                   : "memory");
+      return;
+    }
+    q[1] = r.q[1];
+  }
   q[0] = r.q[0];
-  if constexpr (sizeof(T) == 4) q[1] = r.q[1];
 }
 
 inline bool known_dtype(int32_t d) {
