@@ -158,8 +158,8 @@ _host = None
 
 
 def host():
-    """The native host plan module (t3st_b200._dfc_host), built first if it
-    is absent (needs g++ and PyTorch's headers)."""
+    """The native host module (t3st_b200._dfc_host), built first if it is
+    absent (needs g++ and PyTorch's headers)."""
     global _host
     if _host is None:
         import importlib
@@ -169,6 +169,9 @@ def host():
         if not os.path.exists(_build.HOST_PATH):
             _build.build_host()
         _host = importlib.import_module("t3st_b200._dfc_host")
+        _host.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in
+                     ("dfc_dropout", "dfc_embedding", "dfc_embedding_grad_scratch_bytes",
+                      "dfc_embedding_grad")), check)
     return _host
 
 

@@ -3,9 +3,10 @@
 - libdfc_b200.so from t3st_b200/csrc/*.cu with nvcc: the kernels behind the
   C ABI of include/dfc_b200.h (no PyTorch headers, CUDA runtime linked
   statically), loaded with ctypes by t3st_b200/_lib.py;
-- _dfc_host (a CPython extension) from t3st_b200/csrc/dfc_host_plan.cpp with
-  g++ against PyTorch's headers: the steady-state host path of
-  DFCAdamW.step(), which calls dfc_mt_step through the C ABI.
+- _dfc_host (a CPython extension) from t3st_b200/csrc/dfc_host_*.cpp with g++
+  against PyTorch's headers: the steady-state host path of DFCAdamW.step() and
+  the host path of the token table and dropout, which call the kernels through
+  the C ABI.
 
     python -m t3st_b200.build            # build what any source is newer than
     python -m t3st_b200.build --force    # rebuild
@@ -26,7 +27,7 @@ REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB_PATH = os.path.join(PKG, "libdfc_b200.so")
-HOST_SRC = os.path.join(CSRC, "dfc_host_plan.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("dfc_host_plan.cpp", "dfc_host_tokens.cpp")]
 HOST_PATH = os.path.join(PKG, "_dfc_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
@@ -63,8 +64,8 @@ def nvcc() -> str:
 
 
 def build_host(force: bool = False) -> str:
-    """Compile the DFCAdamW host plan (CPython extension); return its path."""
-    if not force and not _stale(HOST_PATH, [HOST_SRC, os.path.join(INCLUDE, "dfc_b200.h")]):
+    """Compile the native host paths (CPython extension); return its path."""
+    if not force and not _stale(HOST_PATH, [*HOST_SRCS, os.path.join(INCLUDE, "dfc_b200.h")]):
         return HOST_PATH
     import torch
     from torch.utils import cpp_extension
@@ -76,12 +77,12 @@ def build_host(force: bool = False) -> str:
     tmp = HOST_PATH + f".tmp{os.getpid()}"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{d}" for d in incs], HOST_SRC, "-o", tmp, f"-L{libdir}", f"-Wl,-rpath,{libdir}",
+           *[f"-I{d}" for d in incs], *HOST_SRCS, "-o", tmp, f"-L{libdir}", f"-Wl,-rpath,{libdir}",
            "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError("g++ failed building the DFCAdamW host plan")
+        raise RuntimeError("g++ failed building the native host paths")
     os.replace(tmp, HOST_PATH)
     return HOST_PATH
 

@@ -6,9 +6,11 @@
 //      to 131,072 tokens one cluster of CTAs sorts in its shared memory;
 //   2. sum_kernel: the sorted positions are cut into tiles of K; one thread
 //      holds eight columns of a tile and adds its rows in order in FP32
-//      registers, writing a row of grad at each end of a run.  A run that
-//      crosses tile borders leaves FP32 partial rows in the scratch instead.
-//      The same grid zeroes the rows of an overwritten grad that no token names;
+//      registers, writing a row of grad at each end of a run.  The parts of a
+//      run that crosses tiles are added through shared memory among the tiles
+//      of a CTA, its block; a run that crosses blocks leaves FP32 partial rows
+//      in the scratch.  The same grid zeroes the rows of an overwritten grad
+//      that no token names;
 //   3. join_kernel adds such a run's partial rows in a fixed order.
 // No atomics on floats: the same inputs give the same bits.
 #include <cooperative_groups.h>
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     sort_cluster_kernel(Tokens tk, uint32_t n, int passes, int digit_bits, uint32_t* out_keys,
                         uint32_t* out_pos) {
   constexpr uint32_t kChunk = kClusterThreads * ITEMS;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t warp_own[kClusterWarps], warp_all[kClusterWarps];
   const uint32_t bins = 1u << digit_bits;
   uint2* ordered = reinterpret_cast<uint2*>(smem);
@@ -347,7 +349,8 @@ struct SumArgs {
   float scale;
   int accumulate;
   int wide_dy, wide_grad;  // rows on 32-byte boundaries
-  float* partial;        // 2 rows a tile: a run from before it, a run that goes on behind it
+  int64_t block;         // positions of a CTA's tiles
+  float* partial;        // 2 rows a block: a run from before it, a run that goes on behind it
   int64_t partial_pitch; // dim rounded up to 8
   const uint8_t* named;  // one byte per row of an overwritten grad
   DropArgs drop;
@@ -364,37 +367,39 @@ __device__ __forceinline__ void row8(const T* at, int64_t c, int64_t dim, int wi
   }
 }
 
-// v[u][j] = element e[u] + j kept ? v[u][j] : 0 (the scale is applied to the sum).
-template <int N, bool VEC>
-__device__ __forceinline__ void mask8(float (&v)[N][8], const int64_t (&e)[N], const DropArgs& a,
-                                      const DropKey& k) {
-  uint64_t g[N];
-  uint4 w[N];
+// The fates of the eight elements e[u] .. e[u] + 7 for two rows.  VEC: e is a
+// multiple of eight, they are one group; otherwise they may reach into the next.
+template <bool VEC>
+struct Fates {
+  uint4 w[2];
+
+  __device__ __forceinline__ void set(const int64_t (&e)[2], const DropArgs& a, const DropKey& k) {
+    uint64_t g[2] = {static_cast<uint64_t>(e[0]) >> 3, static_cast<uint64_t>(e[1]) >> 3};
+    drop_words<2>(g, a, k, w);
+    if constexpr (!VEC) {  // w[u].x: one bit per element
+      uint32_t bits[2] = {0u, 0u};
 #pragma unroll
-  for (int u = 0; u < N; ++u) g[u] = static_cast<uint64_t>(e[u]) >> 3;
-  drop_words<N>(g, a, k, w);
-  if constexpr (VEC) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int u = 0; u < N; ++u)
+        for (int j = 0; j < 8; ++j) bits[u] |= kept(w[u], j, a.cmp) ? 1u << j : 0u;
+      ++g[0];
+      ++g[1];
+      drop_words<2>(g, a, k, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[u][j] = kept(w[u], j, a.cmp) ? v[u][j] : 0.0f;
-  } else {
-    uint4 x[N];  // the eight elements reach into the next group
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-    for (int u = 0; u < N; ++u) ++g[u];
-    drop_words<N>(g, a, k, x);
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        bits |= (kept(w[u], j, a.cmp) ? 1u << j : 0u) | (kept(x[u], j, a.cmp) ? 256u << j : 0u);
-      bits >>= e[u] & 7;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[u][j] = (bits >> j) & 1u ? v[u][j] : 0.0f;
+        for (int j = 0; j < 8; ++j) bits[u] |= kept(w[u], j, a.cmp) ? 256u << j : 0u;
+        w[u].x = bits[u] >> (e[u] & 7);
+      }
     }
   }
-}
+
+  // v[j] = kept ? v[j] : 0 (the scale is applied to the sum)
+  __device__ __forceinline__ void apply(int u, const DropArgs& a, float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (VEC ? kept(w[u], j, a.cmp) : (w[u].x >> j) & 1u) ? v[j] : 0.0f;
+  }
+};
 
 template <typename TG, bool VEC>
 __device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t c, float (&v)[8]) {
@@ -416,148 +421,267 @@ __device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t
   }
 }
 
-constexpr int kSumThreads = 128;
+constexpr int kSumThreads = 256;
 constexpr int kSumLanes = 64;  // threads of a tile's slab of 512 columns, at most
-#ifndef DFC_SUM_BLOCKS
-#define DFC_SUM_BLOCKS 1
-#endif
-constexpr int kBatch = 4;
 constexpr int kFillRows = 32;
+// Rows that a thread has on the way: kStages groups of kGroup<T> 16-byte or
+// 32-byte pieces, in shared memory of its own.
+constexpr int kStages = 2;
+template <typename TD>
+constexpr int kGroup = sizeof(TD) == 2 ? 4 : 2;
+constexpr int kRingBytes = kStages * 4 * 16 * kSumThreads;
+constexpr int kPartBytes = 2 * 8 * 4 * kSumThreads;
+constexpr int kZeroBytes = kPartBytes;  // the piece of zeros that fill() copies from
 
-// Zeros for the rows [first, first + rows) that no token names.
+// Zeros for the rows [first, first + rows) that no token names: bulk copies
+// from zeros in shared memory, so that the rate does not depend on how many of
+// this kernel's CTAs an SM holds (stores from registers: 554 us instead of 382
+// for grad-largest's rows at two CTAs of 256 threads per SM).
 template <typename TG, bool VEC>
-__device__ __forceinline__ void fill(const SumArgs& s, int64_t first, int rows) {
+__device__ __forceinline__ void fill(const SumArgs& s, int64_t first, int rows, void* zeros) {
   const int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid & 31;
   const int64_t mine = first + lane;
   const uint32_t empty = __ballot_sync(0xFFFFFFFFu, lane < rows && mine < s.vocab && !s.named[mine]);
-  for (int r = 0; r < rows; ++r) {
-    if (!((empty >> r) & 1u)) continue;
-    TG* row = static_cast<TG*>(s.grad) + (first + r) * s.grad_pitch;
-    if constexpr (VEC) {
-      uint4* q = reinterpret_cast<uint4*>(row);
-      for (int64_t c = tid; c < s.dim * static_cast<int64_t>(sizeof(TG)) / 16; c += kSumThreads)
-        q[c] = make_uint4(0u, 0u, 0u, 0u);
-    } else {
+  if constexpr (VEC) {
+    for (int i = tid; i < kZeroBytes / 16; i += kSumThreads)
+      static_cast<uint4*>(zeros)[i] = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    if (tid < rows && ((empty >> tid) & 1u)) {  // one thread a row
+      char* row = reinterpret_cast<char*>(static_cast<TG*>(s.grad) + mine * s.grad_pitch);
+      const uint32_t from = static_cast<uint32_t>(__cvta_generic_to_shared(zeros));
+      const int64_t bytes = s.dim * static_cast<int64_t>(sizeof(TG));  // a multiple of 16
+      for (int64_t at = 0; at < bytes; at += kZeroBytes)
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(row + at), "r"(from),
+                     "r"(static_cast<uint32_t>(min(bytes - at, static_cast<int64_t>(kZeroBytes))))
+                     : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+  } else {
+    for (int r = 0; r < rows; ++r) {
+      if (!((empty >> r) & 1u)) continue;
+      TG* row = static_cast<TG*>(s.grad) + (first + r) * s.grad_pitch;
       for (int64_t c = tid; c < s.dim; c += kSumThreads) row[c] = from_f32<TG>(0.0f);
     }
   }
 }
 
-template <typename TD>
-struct Batch {
-  uint32_t key[kBatch], pos[kBatch];
-  Raw8<TD> row[kBatch];
-};
-
-// Keys (kNoKey behind hi) and positions of items i .. i + 3; i is a multiple of
-// kBatch and the arrays are allocated in whole tiles.
-__device__ __forceinline__ void batch_ids(const SumArgs& s, int64_t i, int64_t hi, uint4& k4, uint4& p4) {
-  k4 = p4 = make_uint4(kNoKey, kNoKey, kNoKey, kNoKey);
-  if (i >= hi) return;
-  k4 = *reinterpret_cast<const uint4*>(s.keys + i);
-  p4 = *reinterpret_cast<const uint4*>(s.pos + i);
-  if (i + 1 >= hi) k4.y = kNoKey;
-  if (i + 2 >= hi) k4.z = kNoKey;
-  if (i + 3 >= hi) k4.w = kNoKey;
-}
-
-// Their rows' columns c .. c + 7 (none for keys outside the table).
-template <typename TD, bool VEC>
-__device__ __forceinline__ void batch_rows(const SumArgs& s, const TD* dy, int64_t c, const uint4& k4,
-                                           const uint4& p4, Batch<TD>& b) {
-  b.key[0] = k4.x, b.key[1] = k4.y, b.key[2] = k4.z, b.key[3] = k4.w;
-  b.pos[0] = p4.x, b.pos[1] = p4.y, b.pos[2] = p4.z, b.pos[3] = p4.w;
-#pragma unroll
-  for (int u = 0; u < kBatch; ++u) {
-    if (b.key[u] < s.vocab) {
-      const TD* at = dy + b.pos[u] * s.dy_pitch;
-      if constexpr (VEC) {
-        b.row[u] = load8(at, s.wide_dy);
-      } else {
-        float v[8];
-        row8<TD, false>(at, c, s.dim, 0, v);
-        b.row[u] = pack8<TD>(v);
-      }
-    }
+// N keys from position i on (kNoKey behind hi); i is a multiple of N and the
+// arrays are allocated in whole tiles.
+template <int N>
+__device__ __forceinline__ void load_ids(const uint32_t* ids, int64_t i, uint32_t (&v)[N]) {
+  if constexpr (N == 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(ids + i);
+    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+  } else {
+    const uint2 q = *reinterpret_cast<const uint2*>(ids + i);
+    v[0] = q.x, v[1] = q.y;
   }
 }
 
-// CTAs [0, sum_ctas): blockDim.y units, each a slab of 8 * blockDim.x columns
-// of a tile.  CTAs behind them: fill_rows rows each.
+// The rows of a tile, columns c .. c + 7, group by group.
+template <typename TD, typename TG, bool VEC>
+struct Rows {
+  static constexpr int N = kGroup<TD>;
+  const SumArgs& s;
+  const TD* dy;  // column c of row 0
+  int64_t c, hi;
+  uint32_t ring;  // this thread's slot of the first stage
+
+  // Rows of the group at i go on their way into stage `stage`.  Rows of an
+  // accumulated grad that the ends of its runs will read are brought into L2.
+  __device__ __forceinline__ void request(int64_t i, int stage) const {
+    if (VEC && i < hi) {
+      uint32_t key[N], pos[N];
+      load_ids<N>(s.keys, i, key);
+      load_ids<N>(s.pos, i, pos);
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        if (i + u < hi && key[u] < s.vocab) {
+          const TD* from = dy + pos[u] * s.dy_pitch;
+          const uint32_t to = ring + (stage * N + u) * (8 * sizeof(TD) * kSumThreads);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+          if constexpr (sizeof(TD) == 4)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * kSumThreads), "l"(from + 4)
+                         : "memory");
+          if (s.accumulate && (u == 0 || key[u] != key[u - 1]))
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const TG*>(s.grad) + key[u] * s.grad_pitch + c));
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  __device__ __forceinline__ void arrived() const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+  }
+
+  __device__ __forceinline__ void get(int stage, int u, uint32_t pos, float (&v)[8]) const {
+    if constexpr (VEC) {
+      Raw8<TD> r;
+      const uint32_t at = ring + (stage * N + u) * (8 * sizeof(TD) * kSumThreads);
+      shared16(at, r.q[0]);
+      if constexpr (sizeof(TD) == 4) shared16(at + 16 * kSumThreads, r.q[1]);
+      unpack8<TD>(r, v);
+    } else {
+      row8<TD, false>(dy + pos * s.dy_pitch, c, s.dim, 0, v);
+    }
+  }
+
+  __device__ __forceinline__ static void shared16(uint32_t at, uint4& q) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                 : "r"(at)
+                 : "memory");
+  }
+};
+
+__device__ __forceinline__ void store8_shared(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+template <typename TG>
+__device__ __forceinline__ void put_one(const SumArgs& s, uint32_t key, int64_t c, float sum) {
+  TG* at = static_cast<TG*>(s.grad) + key * s.grad_pitch + c;
+  float v = __fmul_rn(sum, s.scale);
+  if (s.accumulate) v = __fadd_rn(to_f32(*at), v);
+  *at = from_f32<TG>(v);
+}
+
+// What a tile leaves for the sums across tiles: the row its first run adds to
+// (it began before the tile), whether that run goes on behind the tile too, and
+// the row of a last run that begins in the tile and goes on behind it.
+struct Ends {
+  uint32_t head, tail;  // kNoKey: none
+  int through;
+};
+constexpr int kSumSmem = kPartBytes + kRingBytes + static_cast<int>(sizeof(Ends)) * kSumThreads;
+constexpr int kSumCtas = 3;  // per SM
+
+// CTAs [0, sum_ctas): blockDim.y tiles, one after the other, of a slab of
+// 8 * blockDim.x columns.  CTAs behind them: fill_rows rows each.
 template <typename TD, typename TG, bool DROP, bool VEC>
-__global__ void __launch_bounds__(kSumThreads, DFC_SUM_BLOCKS) sum_kernel(SumArgs s, uint32_t slabs, uint32_t sum_ctas,
-                                                          int fill_rows) {
+__global__ void __launch_bounds__(kSumThreads, kSumCtas)
+    sum_kernel(SumArgs s, uint32_t slabs, uint32_t sum_ctas, int fill_rows) {
+  extern __shared__ __align__(128) unsigned char smem[];  // kSumSmem bytes
+  float* part = reinterpret_cast<float*>(smem);            // [head, tail][tile][column]
+  Ends* ends = reinterpret_cast<Ends*>(smem + kPartBytes + kRingBytes);
   let_next_start();
   wait_for_previous();
   if (blockIdx.x >= sum_ctas) {
-    fill<TG, VEC>(s, static_cast<int64_t>(blockIdx.x - sum_ctas) * fill_rows, fill_rows);
+    fill<TG, VEC>(s, static_cast<int64_t>(blockIdx.x - sum_ctas) * fill_rows, fill_rows, smem);
     return;
   }
-  const uint32_t unit = blockIdx.x * blockDim.y + threadIdx.y;
-  const int64_t tile = unit / slabs;
-  const int64_t c = 8ll * ((unit % slabs) * blockDim.x + threadIdx.x);
-  const int64_t lo = tile * s.tile;
-  if (c >= s.dim || lo >= s.n) return;
+  const int64_t block = blockIdx.x / slabs;
+  const int64_t c0 = 8ll * (blockIdx.x % slabs) * blockDim.x;
+  const int64_t c = c0 + 8ll * threadIdx.x;
+  const int64_t lo = block * s.block + static_cast<int64_t>(threadIdx.y) * s.tile;
   const int64_t hi = min(lo + s.tile, s.n);
-  DropKey k{};
-  if (DROP) k = drop_key(s.drop);
-  const TD* dy = static_cast<const TD*>(s.dy) + c;
-  const uint32_t before = lo > 0 ? s.keys[lo - 1] : kNoKey;
-  const uint32_t behind = hi < s.n ? s.keys[hi] : kNoKey;
-  float acc[8];
-  uint32_t run = kNoKey;
-  bool first = true;  // no row of the tile has ended a run yet
-  // Three batches are under way: the rows of one are added while those of the
-  // next are on their way and the positions of the one after it are read.
-  Batch<TD> now, next;
-  uint4 k4, p4;
-  batch_ids(s, lo, hi, k4, p4);
-  batch_rows<TD, VEC>(s, dy, c, k4, p4, now);
-  batch_ids(s, lo + kBatch, hi, k4, p4);
-  for (int64_t i = lo; i < hi; i += kBatch) {
-    batch_rows<TD, VEC>(s, dy, c, k4, p4, next);
-    batch_ids(s, i + 2 * kBatch, hi, k4, p4);
-    float v[kBatch][8];
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  Ends mine{kNoKey, kNoKey, 0};
+  if (lo < hi && c < s.dim) {
+    constexpr int N = kGroup<TD>;
+    DropKey k{};
+    if (DROP) k = drop_key(s.drop);
+    const Rows<TD, TG, VEC> rows{s, static_cast<const TD*>(s.dy) + c, c, hi,
+                                 static_cast<uint32_t>(__cvta_generic_to_shared(smem + kPartBytes)) + 16 * tid};
+    const uint32_t before = lo > 0 ? s.keys[lo - 1] : kNoKey;
+    const uint32_t behind = hi < s.n ? s.keys[hi] : kNoKey;
+    float acc[8];
+    uint32_t run = kNoKey;
+    bool first = true;  // no run of the tile has ended yet
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) unpack8<TD>(now.row[u], v[u]);
-    if (DROP) {
-      int64_t e[kBatch];
+    for (int g = 0; g < kStages; ++g) rows.request(lo + g * N, g);
+    int stage = 0;
+    for (int64_t i = lo; i < hi; i += N) {
+      rows.arrived();
+      uint32_t key[N], pos[N];
+      load_ids<N>(s.keys, i, key);
+      if (DROP || !VEC) load_ids<N>(s.pos, i, pos);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) e[u] = now.pos[u] * s.dim + c;
-      mask8<kBatch, VEC>(v, e, s.drop, k);
-    }
+      for (int u = 0; u < N; u += 2) {
+        Fates<VEC> fates;
+        if (DROP) fates.set({pos[u] * s.dim + c, pos[u + 1] * s.dim + c}, s.drop, k);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const uint32_t key = now.key[u];
-      if (key >= s.vocab) continue;
-      if (key == run) {
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t id = key[u + h];
+          if (i + u + h >= hi || id >= s.vocab) continue;
+          float v[8];
+          rows.get(stage, u + h, pos[u + h], v);
+          if (DROP) fates.apply(h, s.drop, v);
+          if (id == run) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = __fadd_rn(acc[j], v[u][j]);
-      } else {
-        if (run != kNoKey) {
-          if (first && run == before)
-            store8(s.partial + 2 * tile * s.partial_pitch + c, pack8<float>(acc), 1);
-          else
-            put_row8<TG, VEC>(s, run, c, acc);
-          first = false;
+            for (int j = 0; j < 8; ++j) acc[j] = __fadd_rn(acc[j], v[j]);
+          } else {
+            if (run != kNoKey) {
+              if (first && run == before) {
+                store8_shared(part + 8 * tid, acc);
+                mine.head = run;
+              } else {
+                put_row8<TG, VEC>(s, run, c, acc);
+              }
+              first = false;
+            }
+            run = id;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] = v[j];
+          }
         }
-        run = key;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = v[u][j];
+      }
+      rows.request(i + kStages * N, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    if (run != kNoKey) {
+      if (first && run == before) {
+        store8_shared(part + 8 * tid, acc);
+        mine.head = run;
+        mine.through = run == behind;
+      } else if (run == behind) {
+        store8_shared(part + 8 * (kSumThreads + tid), acc);
+        mine.tail = run;
+      } else {
+        put_row8<TG, VEC>(s, run, c, acc);
       }
     }
-    now = next;
   }
-  if (run == kNoKey) return;
-  if (first && run == before)
-    store8(s.partial + 2 * tile * s.partial_pitch + c, pack8<float>(acc), 1);
-  else if (run == behind)
-    store8(s.partial + (2 * tile + 1) * s.partial_pitch + c, pack8<float>(acc), 1);
-  else
-    put_row8<TG, VEC>(s, run, c, acc);
+  if (threadIdx.x == 0) ends[threadIdx.y] = mine;
+  __syncthreads();
+  // Runs across tiles: one thread per column goes through the tiles in order.
+  const int columns = 8 * blockDim.x;
+  for (int col = threadIdx.y * blockDim.x + threadIdx.x; col < columns; col += kSumThreads) {
+    if (c0 + col >= s.dim) break;
+    float acc = 0.0f;
+    bool from_before = false, open = false;
+    for (int t = 0; t < blockDim.y; ++t) {
+      const Ends e = ends[t];
+      if (e.head != kNoKey) {
+        const float x = part[t * columns + col];
+        if (t == 0) {
+          acc = x;
+          from_before = open = true;
+        } else {
+          acc = __fadd_rn(acc, x);
+        }
+        if (!e.through) {
+          if (from_before)
+            s.partial[2 * block * s.partial_pitch + c0 + col] = acc;
+          else
+            put_one<TG>(s, e.head, c0 + col, acc);
+          open = from_before = false;
+        }
+      }
+      if (e.tail != kNoKey) {
+        acc = part[8 * kSumThreads + t * columns + col];
+        open = true;
+      }
+    }
+    if (open) s.partial[(2 * block + (from_before ? 0 : 1)) * s.partial_pitch + c0 + col] = acc;
+  }
 }
 
-// ---- 3. runs that cross tile borders --------------------------------------------
+// ---- 3. runs that cross blocks ----------------------------------------------------
 constexpr int kJoinLanes = 64;
 constexpr int kJoinParts = 4;
 constexpr int kJoinThreads = kJoinLanes * kJoinParts;
@@ -569,24 +693,24 @@ __device__ __forceinline__ void add4(float4& a, const float4& b) {
   a.w = __fadd_rn(a.w, b.w);
 }
 
-// Tile blockIdx.x, if a run begins in it and goes on behind it; 4 columns per
+// Block blockIdx.x, if a run begins in it and goes on behind it; 4 columns per
 // lane.  Part q adds the run's partial rows q, q + 4, ...; part 0 the four sums.
 template <typename TG>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(SumArgs s) {
   __shared__ float4 sums[kJoinParts][kJoinLanes];
   let_next_start();
   wait_for_previous();
-  const int64_t tile = blockIdx.x;
-  const int64_t lo = tile * s.tile, hi = lo + s.tile;
+  const int64_t block = blockIdx.x;
+  const int64_t lo = block * s.block, hi = lo + s.block;
   if (hi >= s.n) return;
   const uint32_t key = s.keys[hi - 1], behind = s.keys[hi];
   const uint32_t before = lo > 0 ? s.keys[lo - 1] : kNoKey;
   if (key >= s.vocab || behind != key || before == key) return;
-  // the tiles behind this one whose first item has the key are consecutive
+  // the blocks behind this one whose first item has the key are consecutive
   const int tid = threadIdx.y * kJoinLanes + threadIdx.x;
   int64_t more = 0;
   for (int found = kJoinThreads; found == kJoinThreads; more += found) {
-    const int64_t i = (tile + 1 + more + tid) * s.tile;
+    const int64_t i = (block + 1 + more + tid) * s.block;
     found = __syncthreads_count(i < s.n && s.keys[i] == key);
   }
   const int64_t c = 4 * (static_cast<int64_t>(blockIdx.y) * kJoinLanes + threadIdx.x);
@@ -595,7 +719,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(SumArgs s) {
   if (on) {
 #pragma unroll 4
     for (int64_t j = threadIdx.y; j <= more; j += kJoinParts) {
-      const int64_t row = j == 0 ? 2 * tile + 1 : 2 * (tile + j);
+      const int64_t row = j == 0 ? 2 * block + 1 : 2 * (block + j);
       add4(acc, *reinterpret_cast<const float4*>(s.partial + row * s.partial_pitch + c));
     }
   }
@@ -605,49 +729,41 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(SumArgs s) {
 #pragma unroll
   for (int q = 1; q < kJoinParts; ++q) add4(acc, sums[q][threadIdx.x]);
   const float f[4] = {acc.x, acc.y, acc.z, acc.w};
-  TG* row = static_cast<TG*>(s.grad) + key * s.grad_pitch;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (c + j < s.dim) {
-      float v = __fmul_rn(f[j], s.scale);
-      if (s.accumulate) v = __fadd_rn(to_f32(row[c + j]), v);
-      row[c + j] = from_f32<TG>(v);
-    }
-  }
+  for (int j = 0; j < 4; ++j)
+    if (c + j < s.dim) put_one<TG>(s, key, c + j, f[j]);
 }
 
 // ---- host -------------------------------------------------------------------------
-// Threads of a slab and slabs of a row.
+// Threads of a slab, slabs of a row, tiles of a CTA.
 struct Shape {
   int lanes;
   int64_t slabs;
+  int tiles;
 };
 
 Shape shape(int64_t dim) {
   const int64_t need = (dim + 7) / 8;
   int lanes = 1;
   while (lanes < need && lanes < kSumLanes) lanes *= 2;
-  return {lanes, (need + lanes - 1) / lanes};
+  return {lanes, (need + lanes - 1) / lanes, kSumThreads / lanes};
 }
 
-// K: enough units for every SM, no more partial rows than that takes.
-#ifndef DFC_UNITS
-#define DFC_UNITS 2400
-#endif
-constexpr int kMinTile = 8, kMaxTile = 256, kUnits = DFC_UNITS;
+// K: enough threads for every SM, no more ends of tiles than that takes.
+constexpr int kMinTile = 8, kMaxTile = 256;
+constexpr int64_t kThreadsWanted = 300000;
 
 int tile_tokens(int64_t n, int64_t dim) {
   const Shape sh = shape(dim);
-  const int64_t units_per_token = sh.slabs * sh.lanes;  // in threads
   int tile = kMinTile;
-  while (tile < kMaxTile && tile * int64_t{kUnits} * kSumLanes < n * units_per_token) tile *= 2;
+  while (tile < kMaxTile && tile * kThreadsWanted < n * sh.slabs * sh.lanes) tile *= 2;
   return tile;
 }
 
 struct Layout {
   int64_t sort_tiles;
   int passes, digit_bits, tile;
-  int64_t partial_pitch;
+  int64_t block, partial_pitch;
   size_t keys[2], pos[2], hist, named, partial, bytes;
 };
 
@@ -659,6 +775,7 @@ Layout layout(int64_t n, int64_t vocab, int64_t dim) {
   l.digit_bits = (bits + l.passes - 1) / l.passes;
   l.sort_tiles = (n + kSortTile - 1) / kSortTile;
   l.tile = tile_tokens(n, dim);
+  l.block = int64_t{l.tile} * shape(dim).tiles;
   l.partial_pitch = (dim + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&at](int64_t bytes) {
@@ -675,7 +792,7 @@ Layout layout(int64_t n, int64_t vocab, int64_t dim) {
   }
   if (!cluster) l.hist = take(l.sort_tiles * (int64_t{4} << l.digit_bits));
   l.named = take(vocab);
-  l.partial = take(8 * ((n + l.tile - 1) / l.tile) * l.partial_pitch);
+  l.partial = take(8 * ((n + l.block - 1) / l.block) * l.partial_pitch);
   l.bytes = at;
   return l;
 }
@@ -743,10 +860,12 @@ int max_cluster() {
 }
 
 template <typename Kernel, typename... Args>
-cudaError_t launch_next(Kernel kernel, dim3 grid, dim3 block, cudaStream_t st, const Args&... args) {
+cudaError_t launch_next(Kernel kernel, dim3 grid, dim3 block, int smem, cudaStream_t st,
+                        const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -819,21 +938,23 @@ bool sizes_ok(int64_t n, int64_t vocab, int64_t dim) {
 template <typename TD, typename TG, bool DROP, bool VEC>
 int run_sums(const SumArgs& s, cudaStream_t st) {
   const Shape sh = shape(s.dim);
-  const int64_t tiles = (s.n + s.tile - 1) / s.tile;
-  const int subs = kSumThreads / sh.lanes;
-  const int64_t sum_ctas = (tiles * sh.slabs + subs - 1) / subs;
+  const int64_t blocks = (s.n + s.block - 1) / s.block;
+  const int64_t sum_ctas = blocks * sh.slabs;
   const int64_t row_bytes = s.dim * static_cast<int64_t>(sizeof(TG));
-  const int rows = static_cast<int>(std::min<int64_t>(kFillRows, std::max<int64_t>(1, 32768 / row_bytes)));
+  const int rows = static_cast<int>(std::min<int64_t>(kFillRows, std::max<int64_t>(1, 65536 / row_bytes)));
   const int64_t fill_ctas = s.accumulate ? 0 : (s.vocab + rows - 1) / rows;
   if (sum_ctas + fill_ctas == 0) return DFC_OK;
-  cudaError_t e = launch_next(sum_kernel<TD, TG, DROP, VEC>, dim3(static_cast<unsigned>(sum_ctas + fill_ctas)),
-                              dim3(sh.lanes, subs), st, s, static_cast<uint32_t>(sh.slabs),
+  cudaError_t e = cudaFuncSetAttribute(sum_kernel<TD, TG, DROP, VEC>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSumSmem);
+  if (e != cudaSuccess) return failed(e);
+  e = launch_next(sum_kernel<TD, TG, DROP, VEC>, dim3(static_cast<unsigned>(sum_ctas + fill_ctas)),
+                              dim3(sh.lanes, sh.tiles), kSumSmem, st, s, static_cast<uint32_t>(sh.slabs),
                               static_cast<uint32_t>(sum_ctas), rows);
-  if (e == cudaSuccess && tiles > 1)
+  if (e == cudaSuccess && blocks > 1)
     e = launch_next(join_kernel<TG>,
-                    dim3(static_cast<unsigned>(tiles - 1),
+                    dim3(static_cast<unsigned>(blocks - 1),
                          static_cast<unsigned>((s.dim + 4 * kJoinLanes - 1) / (4 * kJoinLanes))),
-                    dim3(kJoinLanes, kJoinParts), st, s);
+                    dim3(kJoinLanes, kJoinParts), 0, st, s);
   return e == cudaSuccess ? launch_status() : failed(e);
 }
 
@@ -897,6 +1018,7 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   s.named = named;
   s.n = n_tokens;
   s.tile = l.tile;
+  s.block = l.block;
   s.dy = dy;
   s.dy_pitch = dy_pitch;
   s.grad = grad;

@@ -33,6 +33,11 @@
 
 #include "dfc_b200.h"
 
+// Token-table and dropout entry points (dfc_host_tokens.cpp).
+using FastCall = PyObject*(PyObject*, PyObject* const*, Py_ssize_t);
+FastCall dfc_py_bind, dfc_py_dropout, dfc_py_embedding, dfc_py_embedding_grad, dfc_py_check_tokens,
+    dfc_py_nn_dropout, dfc_py_nn_embedding;
+
 namespace {
 
 using LaunchFn = int (*)(const DfcSegment*, int32_t, const DfcHyper*, int32_t, int32_t,
@@ -469,13 +474,30 @@ PyMethodDef plan_methods[] = {
 
 PyTypeObject PlanType = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
+PyMethodDef fast(const char* name, FastCall* f, const char* doc) {
+  return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, doc};
+}
+
 PyMethodDef module_methods[] = {
     {"hyper_row", py_hyper_row, METH_VARARGS,
      "hyper_row(lr, beta1, beta2, eps, weight_decay, step) -> the FP32 hyper set"},
+    fast("bind", dfc_py_bind, "bind(dfc_dropout, dfc_embedding, dfc_embedding_grad_scratch_bytes, "
+                              "dfc_embedding_grad, check): addresses and the status check"),
+    fast("dropout", dfc_py_dropout, "dropout(x, out, p, seed, offset, state, residual) -> out"),
+    fast("embedding", dfc_py_embedding,
+         "embedding(tokens, table, out, scale, p, seed, offset, state) -> out"),
+    fast("embedding_grad", dfc_py_embedding_grad,
+         "embedding_grad(tokens, dy, grad, scale, padding_idx, p, seed, offset, state, accumulate) -> grad"),
+    fast("check_tokens", dfc_py_check_tokens, "check_tokens(device index)"),
+    fast("nn_dropout", dfc_py_nn_dropout, "nn_dropout(x, p, seed, offset, state, residual) -> y"),
+    fast("nn_embedding", dfc_py_nn_embedding,
+         "nn_embedding(tokens, weight, scale, padding_idx, p, seed, offset, state, out_dtype, "
+         "grad_in_place) -> rows"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_dfc_host",
-                          "Native steady-state host path of DFCAdamW.step().", -1,
+                          "Native host paths: DFCAdamW.step() in the steady state, the token table and "
+                          "dropout.", -1,
                           module_methods};
 
 }  // namespace

@@ -7,8 +7,6 @@ the tensors' device.  Nothing here falls back to PyTorch arithmetic.
 
 from __future__ import annotations
 
-import ctypes
-import struct
 from typing import Sequence
 
 import numpy as np
@@ -176,103 +174,16 @@ def clip_coef(stats: torch.Tensor, n: int, max_norm: float) -> torch.Tensor:
 
 
 # ---- token table and dropout -------------------------------------------------
-_U64 = (1 << 64) - 1
-_PACK_DROPOUT = struct.Struct("<QQQd")  # DfcDropout
-assert _PACK_DROPOUT.size == _lib.DROPOUT_DTYPE.itemsize
-
-# one int per device, in pinned host memory that the device writes: set by a
-# token outside the table, read (without waiting) by the next call there
-_token_flags: dict[int, tuple[torch.Tensor, ctypes.c_int32]] = {}
-
-
-def _dropout_arg(p: float, seed: int, offset: int, state: torch.Tensor | None,
-                 dev: torch.device) -> bytes | None:
-    p = float(p)
-    if not 0.0 <= p <= 1.0:
-        raise ValueError("dropout probability must be in [0, 1]")
-    if p == 0.0:
-        return None
-    if state is None:
-        return _PACK_DROPOUT.pack(seed & _U64, offset & _U64, 0, p)
-    if state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous():
-        raise TypeError("the generator state must be two contiguous int64 values (seed, offset)")
-    if state.device != dev:
-        raise RuntimeError("all tensors of one call must share a device")
-    return _PACK_DROPOUT.pack(0, offset & _U64, state.data_ptr(), p)
-
-
-def _code(t: torch.Tensor, what: str) -> int:
-    code = DTYPE_CODES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{what} must be FP32, bf16 or fp16")
-    return code
-
+# checked, launched and given scratch by the native host module
 
 def dropout(x: torch.Tensor, out: torch.Tensor, p: float, seed: int = 0, offset: int = 0, *,
             residual: torch.Tensor | None = None, state: torch.Tensor | None = None) -> torch.Tensor:
     """out = residual + (kept ? x / (1 - p) : 0); see dfc_dropout in
-    include/dfc_b200.h for the mask.  ``out`` may be ``x`` or ``residual``.
-    ``state``: a CUDA int64 tensor (seed, offset), read when the kernel runs;
-    the seed is then its first word and the offset its second plus ``offset``."""
-    ts = (x, out) if residual is None else (x, out, residual)
-    dev = _need_cuda(*ts)
-    code = _code(x, "x")
-    for t in ts:
-        if t.dtype != x.dtype:
-            raise TypeError("x, out and residual must share a dtype")
-        if t.shape != x.shape:
-            raise ValueError("shapes differ")
-        if not t.is_contiguous():
-            raise ValueError("tensors must be contiguous")
-    arg = _dropout_arg(p, seed, offset, state, dev)
-    with torch.cuda.device(dev):
-        _lib.check("dfc_dropout", _lib.lib().dfc_dropout(
-            x.data_ptr(), residual.data_ptr() if residual is not None else None, out.data_ptr(),
-            x.numel(), code, arg, _stream(dev)))
-    return out
-
-
-def _token_flag(dev: torch.device) -> int:
-    """Address of the device's token flag; raises if an earlier call set it."""
-    index = dev.index
-    entry = _token_flags.get(index)
-    if entry is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("call the token-table operators once on this device before "
-                               "capturing them: the first call allocates pinned memory")
-        t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-        entry = _token_flags[index] = (t, ctypes.c_int32.from_address(t.data_ptr()))
-    if entry[1].value:
-        check_tokens(dev)
-    return entry[0].data_ptr()
-
-
-def check_tokens(device) -> None:
-    """Raise IndexError if a token-table call on this device, among those
-    whose kernels have finished, met a token outside its table (the lookup
-    gave NaN rows, the gradient left the token out).  The calls themselves
-    check it on entry, without waiting; after a synchronize this covers all."""
-    index = torch.device(device).index
-    entry = _token_flags.get(torch.cuda.current_device() if index is None else index)
-    if entry is not None and entry[1].value:
-        entry[1].value = 0
-        raise IndexError("an earlier call was given a token outside [0, vocab): "
-                         "its rows are NaN, its gradient lacks those tokens")
-
-
-def _tokens_arg(tokens: torch.Tensor) -> int:
-    if tokens.dtype not in (torch.int32, torch.int64):
-        raise TypeError("tokens must be int32 or int64")
-    if not tokens.is_contiguous():
-        raise ValueError("tokens must be contiguous")
-    return tokens.element_size()
-
-
-def _rows(t: torch.Tensor, what: str) -> int:
-    """Elements between the rows of a matrix whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be a matrix with contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    include/dfc_b200.h for the mask.  ``out`` may be ``x`` or ``residual``,
+    and must not overlap them otherwise.  ``state``: a CUDA int64 tensor (seed,
+    offset), read when the kernel runs; the seed is then its first word and the
+    offset its second plus ``offset``."""
+    return _lib.host().dropout(x, out, p, seed, offset, state, residual)
 
 
 def embedding(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor, *, scale: float = 1.0,
@@ -282,21 +193,7 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor, *, s
     tokens.numel() rows.  Dropout as in :func:`dropout` over out's elements.
     A token outside the table makes its row NaN, and a later call raise
     IndexError (:func:`check_tokens`)."""
-    dev = _need_cuda(tokens, table, out)
-    wide = _tokens_arg(tokens)
-    pitch = _rows(table, "table")
-    vocab, dim = table.shape
-    if out.numel() != tokens.numel() * dim or (out.numel() and out.shape[-1] != dim):
-        raise ValueError("out must hold one row of the table's width per token")
-    if not out.is_contiguous():
-        raise ValueError("out must be contiguous")
-    codes = _code(table, "table"), _code(out, "out")
-    arg = _dropout_arg(p, seed, offset, state, dev)
-    with torch.cuda.device(dev):
-        _lib.check("dfc_embedding", _lib.lib().dfc_embedding(
-            tokens.data_ptr(), wide, tokens.numel(), table.data_ptr(), codes[0], pitch, vocab, dim,
-            float(scale), out.data_ptr(), codes[1], arg, _token_flag(dev), _stream(dev)))
-    return out
+    return _lib.host().embedding(tokens, table, out, scale, p, seed, offset, state)
 
 
 def embedding_grad(tokens: torch.Tensor, dy: torch.Tensor, grad: torch.Tensor, *,
@@ -308,29 +205,14 @@ def embedding_grad(tokens: torch.Tensor, dy: torch.Tensor, grad: torch.Tensor, *
     same bits).  ``dy``: one row per token; ``grad``: one row per table row.
     ``accumulate``: add to grad, touching only rows that occur; otherwise
     grad is overwritten, rows that do not occur with zeros."""
-    dev = _need_cuda(tokens, dy, grad)
-    wide = _tokens_arg(tokens)
-    n = tokens.numel()
-    dy_pitch, grad_pitch = _rows(dy, "dy"), _rows(grad, "grad")
-    vocab, dim = grad.shape
-    if dy.shape[0] != n or dy.shape[1] != dim:
-        raise ValueError("dy must hold one row of grad's width per token")
-    if grad_pitch < dim:
-        raise ValueError("grad's rows overlap")
-    codes = _code(dy, "dy"), _code(grad, "grad")
-    if padding_idx is None:
-        padding_idx = -1
-    elif not -vocab <= padding_idx < vocab:
-        raise ValueError("padding_idx must be within the table")
-    elif padding_idx < 0:
-        padding_idx += vocab
-    arg = _dropout_arg(p, seed, offset, state, dev)
-    lib = _lib.lib()
-    with torch.cuda.device(dev):
-        nbytes = lib.dfc_embedding_grad_scratch_bytes(n, vocab, dim)
-        scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        _lib.check("dfc_embedding_grad", lib.dfc_embedding_grad(
-            tokens.data_ptr(), wide, n, dy.data_ptr(), codes[0], dy_pitch, grad.data_ptr(),
-            codes[1], grad_pitch, vocab, dim, float(scale), padding_idx, int(accumulate), arg,
-            _token_flag(dev), scratch.data_ptr(), nbytes, _stream(dev)))
-    return grad
+    return _lib.host().embedding_grad(tokens, dy, grad, scale, padding_idx, p, seed, offset, state,
+                                      accumulate)
+
+
+def check_tokens(device) -> None:
+    """Raise IndexError if a token-table call on this device, among those
+    whose kernels have finished, met a token outside its table (the lookup
+    gave NaN rows, the gradient left the token out).  The calls themselves
+    check it on entry, without waiting; after a synchronize this covers all."""
+    index = torch.device(device).index
+    _lib.host().check_tokens(torch.cuda.current_device() if index is None else index)

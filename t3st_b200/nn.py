@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import torch
 
-from . import kernels
+from . import _lib
 
 __all__ = ["CounterRng", "Dropout", "Embedding", "dropout", "embedding"]
 
@@ -58,30 +58,11 @@ class CounterRng(torch.nn.Module):
         self.state[1:].add_(_SITES)
 
 
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset, state):
-        ctx.args = p, seed, offset
-        ctx.save_for_backward(state)
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
-        return kernels.dropout(x.contiguous(), y, p, seed, offset, state=state,
-                               residual=None if residual is None else residual.contiguous())
-
-    @staticmethod
-    def backward(ctx, dy):
-        (state,) = ctx.saved_tensors
-        p, seed, offset = ctx.args
-        dx = _Dropout.apply(dy, None, p, seed, offset, state) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
-
-
 def _generator(seed):
     """(seed, state) of a seed argument: an int, a CounterRng or its tensor."""
-    if isinstance(seed, CounterRng):
-        return 0, seed.state
-    if isinstance(seed, torch.Tensor):
-        return 0, seed
-    return int(seed), None
+    if isinstance(seed, int):
+        return seed, None
+    return 0, seed.state if isinstance(seed, CounterRng) else seed
 
 
 def dropout(x: torch.Tensor, p: float, *, seed=0, offset: int = 0,
@@ -92,37 +73,7 @@ def dropout(x: torch.Tensor, p: float, *, seed=0, offset: int = 0,
     int64 tensor (seed, offset).  x: FP32, bf16 or fp16, any strides (the
     result is contiguous); residual: x's shape and dtype."""
     seed, state = _generator(seed)
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("residual must have x's shape and dtype")
-    return _Dropout.apply(x, residual, float(p), seed, int(offset), state)
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, tokens, weight, scale, padding_idx, p, seed, offset, state, out_dtype,
-                grad_in_place):
-        tokens = tokens.contiguous()
-        ctx.args = scale, padding_idx, p, seed, offset
-        ctx.table = weight.shape, weight.dtype
-        ctx.leaf = weight if grad_in_place else None
-        ctx.save_for_backward(tokens, state)
-        out = torch.empty(*tokens.shape, weight.shape[1], dtype=out_dtype, device=weight.device)
-        return kernels.embedding(tokens, weight, out, scale=scale, p=p, seed=seed, offset=offset,
-                                 state=state)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        tokens, state = ctx.saved_tensors
-        scale, padding_idx, p, seed, offset = ctx.args
-        shape, dtype = ctx.table
-        into = ctx.leaf.grad if ctx.leaf is not None else None
-        grad = into if into is not None else torch.empty(shape, dtype=dtype, device=dy.device)
-        if dy.dim() != 2 or (dy.shape[1] > 1 and dy.stride(1) != 1):
-            dy = dy.reshape(-1, shape[1]).contiguous()
-        kernels.embedding_grad(tokens, dy, grad, scale=scale, padding_idx=padding_idx, p=p,
-                               seed=seed, offset=offset, state=state, accumulate=into is not None)
-        return (None, grad if into is None else None) + (None,) * 8
+    return _lib.host().nn_dropout(x, p, seed, offset, state, residual)
 
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
@@ -143,16 +94,9 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
     the weight's gradient do not see it.  The buffer must have been zeroed on
     the stream that ran this forward, or be ordered before it.
     """
-    if weight.dim() != 2:
-        raise ValueError("weight must be a matrix")
-    if padding_idx is not None and not -weight.shape[0] <= padding_idx < weight.shape[0]:
-        raise ValueError("padding_idx must be within the table")
-    if grad_in_place and not weight.is_leaf:
-        raise ValueError("grad_in_place needs a leaf weight")
     seed, state = _generator(seed)
-    return _Embedding.apply(tokens, weight, float(scale), padding_idx, float(p), seed, int(offset),
-                            state, weight.dtype if out_dtype is None else out_dtype,
-                            bool(grad_in_place))
+    return _lib.host().nn_embedding(tokens, weight, scale, padding_idx, p, seed, offset, state,
+                                    out_dtype, grad_in_place)
 
 
 class Dropout(torch.nn.Module):

@@ -455,6 +455,23 @@ def test_in_place_gradient_feeds_the_optimizer(cuda):
         assert torch.equal(a, b)
 
 
+def test_second_derivatives_of_the_lookup(cuda):
+    """The lookup and the table's gradient are each other's gradient."""
+    tok = torch.randint(0, 20, (60,), generator=torch.Generator().manual_seed(5)).cuda()
+    w = randn((20, 24), F32, 1).requires_grad_()
+    dy = randn((60, 24), F32, 2).requires_grad_()
+    v = randn((20, 24), F32, 3)
+    kw = dict(padding_idx=3, p=0.3, seed=8, offset=9)
+    (dw,) = torch.autograd.grad(nn.embedding(tok, w, 2.0, **kw), w, dy, create_graph=True)
+    assert (dw[3] == 0).all()
+    (ddy,) = torch.autograd.grad(dw, dy, v)
+    v[3] = 0
+    assert torch.equal(ddy, nn.embedding(tok, v, 2.0, **kw))
+    w.grad = torch.zeros_like(w)
+    with pytest.raises(RuntimeError):
+        nn.embedding(tok, w, 2.0, grad_in_place=True).sum().backward(create_graph=True)
+
+
 def test_in_place_gradient_accumulates(cuda):
     rng, net = make(True)
     tok = torch.randint(1, 120, (64,), generator=torch.Generator().manual_seed(1)).cuda()

@@ -151,13 +151,20 @@ def test_python_refusals_without_a_gpu():
         with pytest.raises(ValueError):
             nn.Embedding(4, 8, p=p, rng=nn.CounterRng())
         with pytest.raises(ValueError):
-            kernels._dropout_arg(p, 0, 0, None, x.device)
+            nn.dropout(x, p)
     with pytest.raises(TypeError):
-        kernels._dropout_arg(0.5, 0, 0, torch.zeros(2), x.device)
+        nn.dropout(x, 0.5, seed=torch.zeros(2))
     with pytest.raises(TypeError):
-        kernels._dropout_arg(0.5, 0, 0, torch.zeros(3, dtype=torch.int64), x.device)
+        nn.dropout(x, 0.5, seed=torch.zeros(3, dtype=torch.int64))
     with pytest.raises(RuntimeError):
         kernels.embedding_grad(tok, torch.zeros(3, 8), w)
+    with pytest.raises(ValueError):
+        kernels.embedding_grad(tok, torch.zeros(3, 8), w, padding_idx=4)
+    for bad in (dict(seed="1"), dict(offset=1.5), dict(residual=3)):
+        with pytest.raises(TypeError):
+            nn.dropout(x, 0.5, **bad)
+    with pytest.raises(TypeError):
+        nn.embedding(tok, w, out_dtype="bf16")
 
 
 def test_modules_on_the_host():
