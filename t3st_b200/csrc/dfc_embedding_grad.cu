@@ -9,8 +9,8 @@
 //      registers, writing a row of grad at each end of a run.  The parts of a
 //      run that crosses tiles are added through shared memory among the tiles
 //      of a CTA, its block; a run that crosses blocks leaves FP32 partial rows
-//      in the scratch.  The same grid zeroes the rows of an overwritten grad
-//      that no token names;
+//      in the scratch.  More CTAs of the same grid zero the rows of an
+//      overwritten grad that no token names;
 //   3. join_kernel adds such a run's partial rows in a fixed order.
 // No atomics on floats: the same inputs give the same bits.
 #include <cooperative_groups.h>
@@ -34,6 +34,59 @@ __device__ __forceinline__ void let_next_start() {
 }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// ---- rows without a token ---------------------------------------------------
+// Zeros are zeros in every type: rows as bytes.
+struct Fill {
+  char* grad;
+  int64_t pitch, bytes;  // of a row
+  int64_t rows;
+  int per_warp;          // rows of a warp, at most 32
+  int unit;              // 16, 4 or 2: grad, pitch and bytes are multiples of it
+};
+
+constexpr int kZeroBytes = 16384;
+constexpr int kBulkBytes = 512;  // shorter rows are written by ordinary stores
+
+__device__ __forceinline__ void clear_zeros(void* zeros) {
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  for (int i = tid; i < kZeroBytes / 16; i += blockDim.x * blockDim.y)
+    static_cast<uint4*>(zeros)[i] = make_uint4(0u, 0u, 0u, 0u);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// One warp: zeros for the rows first + r whose bit r of `empty` is set.  Long
+// rows are bulk copies from zeros in shared memory, one lane a row, so that the
+// rate does not depend on how many threads an SM holds (16-byte stores: 554 us
+// instead of 370 for 1.8 GB with 512 threads per SM).
+__device__ __forceinline__ void fill_rows(const Fill& f, int64_t first, uint32_t empty, const void* zeros) {
+  const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31;
+  if (f.unit == 16 && f.bytes >= kBulkBytes) {
+    if ((empty >> lane) & 1u) {
+      char* row = f.grad + (first + lane) * f.pitch;
+      const uint32_t from = static_cast<uint32_t>(__cvta_generic_to_shared(zeros));
+      for (int64_t at = 0; at < f.bytes; at += kZeroBytes)
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(row + at), "r"(from),
+                     "r"(static_cast<uint32_t>(min(f.bytes - at, static_cast<int64_t>(kZeroBytes))))
+                     : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    return;
+  }
+  for (; empty; empty &= empty - 1) {
+    char* row = f.grad + (first + __ffs(empty) - 1) * f.pitch;
+    for (int64_t at = static_cast<int64_t>(lane) * f.unit; at < f.bytes; at += 32 * f.unit) {
+      if (f.unit == 16)
+        *reinterpret_cast<uint4*>(row + at) = make_uint4(0u, 0u, 0u, 0u);
+      else if (f.unit == 4)
+        *reinterpret_cast<uint32_t*>(row + at) = 0u;
+      else
+        *reinterpret_cast<uint16_t*>(row + at) = 0;
+    }
+  }
+}
+
+__device__ __forceinline__ void fill_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ---- 1. sort ------------------------------------------------------------------
 constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
@@ -48,7 +101,6 @@ struct Tokens {
   int64_t vocab;
   int64_t padding_idx;
   int32_t* error_flag;
-  uint8_t* named;        // NULL, or one byte per row: a token names it
 };
 
 __device__ __forceinline__ uint32_t token_key(const Tokens& tk, int64_t t) {
@@ -183,7 +235,6 @@ __global__ void __launch_bounds__(kSortThreads)
       const uint32_t at = count[warp][(key[r] >> shift) & (bins - 1)] + rank[r];
       out_keys[at] = key[r];
       out_pos[at] = keys ? pos[i] : static_cast<uint32_t>(i);
-      if (!keys && tk.named && key[r] < tk.vocab) tk.named[key[r]] = 1;
     }
   }
 }
@@ -199,12 +250,9 @@ __global__ void __launch_bounds__(kSortThreads)
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kMaxClusterItems = 8;
-// rows whose `named` bytes the cluster clears itself
-constexpr int64_t kClusterClears = 1 << 20;
-
 template <int ITEMS>
 constexpr size_t cluster_smem(int bins) {
-  return static_cast<size_t>(bins) * (2 * kClusterWarps + 3 * 4) + 2 * 8 * kClusterThreads * ITEMS;
+  return static_cast<size_t>(bins) * (2 * kClusterWarps + 2 + 2 * 4) + 2 * 8 * kClusterThreads * ITEMS;
 }
 
 template <int ITEMS>
@@ -217,10 +265,10 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
   const uint32_t bins = 1u << digit_bits;
   uint2* ordered = reinterpret_cast<uint2*>(smem);
   uint2* arrived = ordered + kChunk;
-  uint32_t* total = reinterpret_cast<uint32_t*>(arrived + kChunk);  // this CTA's items per digit
-  uint32_t* start = total + bins;                                   // their places in `ordered`
+  uint32_t* start = reinterpret_cast<uint32_t*>(arrived + kChunk);  // places of the digits in `ordered`
   uint32_t* move = start + bins;                                    // from there to the whole order
-  uint16_t* count = reinterpret_cast<uint16_t*>(move + bins);       // [warp][digit]
+  uint16_t* total = reinterpret_cast<uint16_t*>(move + bins);       // this CTA's items per digit
+  uint16_t* count = total + bins;                                   // [warp][digit]
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -232,11 +280,6 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
   for (int r = 0; r < ITEMS; ++r) {
     pos[r] = rank * kChunk + item0 + 32 * r;
     key[r] = item0 + 32 * r < here ? token_key(tk, pos[r]) : 0u;
-  }
-  if (tk.named && tk.vocab <= kClusterClears) {
-    const uint32_t words = static_cast<uint32_t>((tk.vocab + 15) / 16);
-    for (uint32_t i = rank * kClusterThreads + threadIdx.x; i < words; i += ctas * kClusterThreads)
-      reinterpret_cast<uint4*>(tk.named)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
   for (int p = 0; p < passes; ++p) {
     const int shift = p * digit_bits;
@@ -261,7 +304,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
       __syncwarp();
     }
     __syncthreads();
-    uint32_t own = 0;
+    uint32_t own = 0, all = 0, earlier = 0;
     if (threadIdx.x < bins) {
 #pragma unroll 16
       for (int w = 0; w < kClusterWarps; ++w) {
@@ -269,10 +312,9 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         count[w * bins + threadIdx.x] = static_cast<uint16_t>(own);
         own += c;
       }
-      total[threadIdx.x] = own;
+      total[threadIdx.x] = static_cast<uint16_t>(own);
     }
     cluster.sync();
-    uint32_t all = 0, earlier = 0;
     if (threadIdx.x < bins) {
 #pragma unroll 8
       for (uint32_t q = 0; q < ctas; ++q) {
@@ -317,8 +359,6 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         } else {
           cluster.map_shared_rank(arrived, at / kChunk)[at % kChunk] = kp;
         }
-        // the bytes were cleared before the barrier of the first pass
-        if (p == 0 && tk.named && kp.x < tk.vocab) tk.named[kp.x] = 1;
       }
     }
     cluster.sync();  // the items have arrived; no CTA leaves while others read its counts
@@ -352,7 +392,6 @@ struct SumArgs {
   int64_t block;         // positions of a CTA's tiles
   float* partial;        // 2 rows a block: a run from before it, a run that goes on behind it
   int64_t partial_pitch; // dim rounded up to 8
-  const uint8_t* named;  // one byte per row of an overwritten grad
   DropArgs drop;
 };
 
@@ -423,7 +462,6 @@ __device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t
 
 constexpr int kSumThreads = 256;
 constexpr int kSumLanes = 64;  // threads of a tile's slab of 512 columns, at most
-constexpr int kFillRows = 32;
 // Rows that a thread has on the way: kStages groups of kGroup<T> 16-byte or
 // 32-byte pieces, in shared memory of its own.
 constexpr int kStages = 2;
@@ -431,40 +469,51 @@ template <typename TD>
 constexpr int kGroup = sizeof(TD) == 2 ? 4 : 2;
 constexpr int kRingBytes = kStages * 4 * 16 * kSumThreads;
 constexpr int kPartBytes = 2 * 8 * 4 * kSumThreads;
-constexpr int kZeroBytes = kPartBytes;  // the piece of zeros that fill() copies from
+static_assert(kPartBytes >= kZeroBytes, "fill_ranges() keeps its zeros there");
 
-// Zeros for the rows [first, first + rows) that no token names: bulk copies
-// from zeros in shared memory, so that the rate does not depend on how many of
-// this kernel's CTAs an SM holds (stores from registers: 554 us instead of 382
-// for grad-largest's rows at two CTAs of 256 threads per SM).
-template <typename TG, bool VEC>
-__device__ __forceinline__ void fill(const SumArgs& s, int64_t first, int rows, void* zeros) {
-  const int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid & 31;
-  const int64_t mine = first + lane;
-  const uint32_t empty = __ballot_sync(0xFFFFFFFFu, lane < rows && mine < s.vocab && !s.named[mine]);
-  if constexpr (VEC) {
-    for (int i = tid; i < kZeroBytes / 16; i += kSumThreads)
-      static_cast<uint4*>(zeros)[i] = make_uint4(0u, 0u, 0u, 0u);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-    if (tid < rows && ((empty >> tid) & 1u)) {  // one thread a row
-      char* row = reinterpret_cast<char*>(static_cast<TG*>(s.grad) + mine * s.grad_pitch);
-      const uint32_t from = static_cast<uint32_t>(__cvta_generic_to_shared(zeros));
-      const int64_t bytes = s.dim * static_cast<int64_t>(sizeof(TG));  // a multiple of 16
-      for (int64_t at = 0; at < bytes; at += kZeroBytes)
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(row + at), "r"(from),
-                     "r"(static_cast<uint32_t>(min(bytes - at, static_cast<int64_t>(kZeroBytes))))
-                     : "memory");
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    }
-  } else {
-    for (int r = 0; r < rows; ++r) {
-      if (!((empty >> r) & 1u)) continue;
-      TG* row = static_cast<TG*>(s.grad) + (first + r) * s.grad_pitch;
-      for (int64_t c = tid; c < s.dim; c += kSumThreads) row[c] = from_f32<TG>(0.0f);
+// The first position at which the sorted keys reach `row` (lanes 0..15 of the
+// warp) or `end` (lanes 16..31): each step, the half-warp's lanes look at the 16
+// ends of equal parts of what is left.
+__device__ __forceinline__ int64_t half_warp_search(const SumArgs& s, int64_t row) {
+  const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31;
+  int64_t a = 0, b = s.n;  // keys before a are below row, keys from b on are not
+  while (__any_sync(0xFFFFFFFFu, a < b)) {
+    const int64_t step = (b - a + 15) / 16, at = a + ((lane & 15) + 1) * step - 1;
+    const bool below = a < b && at < b && s.keys[at] < row;  // one half may be done before the other
+    const int parts = __popc((__ballot_sync(0xFFFFFFFFu, below) >> (lane & 16)) & 0xFFFFu);
+    if (a < b) {
+      const int64_t next = a + parts * step;
+      b = min(b, next + step - 1);
+      a = min(next, b);
     }
   }
+  return a;
+}
+
+// Zeros for those rows of CTA `cta`, f.per_warp a warp, that the sorted keys lack.
+__device__ __forceinline__ void fill_searched(const SumArgs& s, const Fill& f, uint32_t cta, void* zeros) {
+  clear_zeros(zeros);
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid & 31;
+  const int64_t first = (static_cast<int64_t>(cta) * (kSumThreads / 32) + (tid >> 5)) * f.per_warp;
+  const int64_t found = half_warp_search(s, lane < 16 ? first : first + f.per_warp);
+  int64_t a = __shfl_sync(0xFFFFFFFFu, found, 0);
+  const int64_t end = __shfl_sync(0xFFFFFFFFu, found, 16);
+  const int64_t row = first + lane;
+  bool empty = false;
+  if (lane < f.per_warp && row < f.rows) {
+    int64_t b = end;  // the first key >= row lies in [a, end]
+    while (a < b) {
+      const int64_t m = (a + b) / 2;
+      if (s.keys[m] < row)
+        a = m + 1;
+      else
+        b = m;
+    }
+    empty = a == end || s.keys[a] != row;
+  }
+  __syncthreads();  // the zeros
+  fill_rows(f, first, __ballot_sync(0xFFFFFFFFu, empty), zeros);
+  fill_done();
 }
 
 // N keys from position i on (kNoKey behind hi); i is a multiple of N and the
@@ -560,18 +609,19 @@ struct Ends {
 constexpr int kSumSmem = kPartBytes + kRingBytes + static_cast<int>(sizeof(Ends)) * kSumThreads;
 constexpr int kSumCtas = 3;  // per SM
 
-// CTAs [0, sum_ctas): blockDim.y tiles, one after the other, of a slab of
-// 8 * blockDim.x columns.  CTAs behind them: fill_rows rows each.
+// A CTA sums blockDim.y tiles, one after the other, of a slab of 8 * blockDim.x
+// columns; those behind sum_ctas zero rows (in the order of their addresses:
+// spread evenly among the others they took 460 us instead of 420 in all).
 template <typename TD, typename TG, bool DROP, bool VEC>
 __global__ void __launch_bounds__(kSumThreads, kSumCtas)
-    sum_kernel(SumArgs s, uint32_t slabs, uint32_t sum_ctas, int fill_rows) {
+    sum_kernel(SumArgs s, uint32_t slabs, uint32_t sum_ctas, Fill f) {
   extern __shared__ __align__(128) unsigned char smem[];  // kSumSmem bytes
   float* part = reinterpret_cast<float*>(smem);            // [head, tail][tile][column]
   Ends* ends = reinterpret_cast<Ends*>(smem + kPartBytes + kRingBytes);
   let_next_start();
   wait_for_previous();
   if (blockIdx.x >= sum_ctas) {
-    fill<TG, VEC>(s, static_cast<int64_t>(blockIdx.x - sum_ctas) * fill_rows, fill_rows, smem);
+    fill_searched(s, f, blockIdx.x - sum_ctas, smem);
     return;
   }
   const int64_t block = blockIdx.x / slabs;
@@ -764,7 +814,7 @@ struct Layout {
   int64_t sort_tiles;
   int passes, digit_bits, tile;
   int64_t block, partial_pitch;
-  size_t keys[2], pos[2], hist, named, partial, bytes;
+  size_t keys[2], pos[2], hist, partial, bytes;
 };
 
 Layout layout(int64_t n, int64_t vocab, int64_t dim) {
@@ -791,18 +841,17 @@ Layout layout(int64_t n, int64_t vocab, int64_t dim) {
     l.pos[i] = take(4 * whole);
   }
   if (!cluster) l.hist = take(l.sort_tiles * (int64_t{4} << l.digit_bits));
-  l.named = take(vocab);
   l.partial = take(8 * ((n + l.block - 1) / l.block) * l.partial_pitch);
   l.bytes = at;
   return l;
 }
 
 template <int ITEMS>
-cudaLaunchConfig_t cluster_config(int ctas, int digit_bits, cudaStream_t st, cudaLaunchAttribute* attr) {
+cudaLaunchConfig_t cluster_config(int ctas, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kClusterThreads);
-  cfg.dynamicSmemBytes = cluster_smem<ITEMS>(1 << digit_bits);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr->id = cudaLaunchAttributeClusterDimension;
   attr->val.clusterDim.x = ctas;
@@ -824,14 +873,14 @@ cudaError_t allow_cluster() {
 }
 
 template <int ITEMS>
-cudaError_t sort_cluster(const Tokens& tk, int64_t n, int ctas, int passes, int digit_bits,
-                         uint32_t* keys, uint32_t* pos, cudaStream_t st) {
+cudaError_t sort_cluster(const Tokens& tk, int64_t n, int ctas, const Layout& l, uint32_t* keys,
+                         uint32_t* pos, cudaStream_t st) {
   const cudaError_t e = allow_cluster<ITEMS>();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr;
-  const cudaLaunchConfig_t cfg = cluster_config<ITEMS>(ctas, digit_bits, st, &attr);
-  return cudaLaunchKernelEx(&cfg, sort_cluster_kernel<ITEMS>, tk, static_cast<uint32_t>(n), passes,
-                            digit_bits, keys, pos);
+  const cudaLaunchConfig_t cfg = cluster_config<ITEMS>(ctas, cluster_smem<ITEMS>(1 << l.digit_bits), st, &attr);
+  return cudaLaunchKernelEx(&cfg, sort_cluster_kernel<ITEMS>, tk, static_cast<uint32_t>(n), l.passes,
+                            l.digit_bits, keys, pos);
 }
 
 // CTAs of the largest cluster on the current device (read once per device).
@@ -847,7 +896,8 @@ int max_cluster() {
   if (ctas == 0) {
     ctas = 8;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = cluster_config<kMaxClusterItems>(16, kMaxDigitBits, nullptr, &attr);
+    const cudaLaunchConfig_t cfg =
+        cluster_config<kMaxClusterItems>(16, cluster_smem<kMaxClusterItems>(kMaxBins), nullptr, &attr);
     int clusters = 0;
     if (allow_cluster<kMaxClusterItems>() == cudaSuccess &&
         cudaOccupancyMaxActiveClusters(&clusters, sort_cluster_kernel<kMaxClusterItems>, &cfg) == cudaSuccess &&
@@ -881,7 +931,7 @@ int failed(cudaError_t e) {
   return DFC_ERR_CUDA;
 }
 
-// Sorted keys and positions of the tokens (and tk.named): DFC_OK or an error.
+// Sorted keys and positions of the tokens: DFC_OK or an error.
 int sort_tokens(const Tokens& tk, int64_t n, const Layout& l, char* scratch, const uint32_t** keys_out,
                 const uint32_t** pos_out, cudaStream_t st) {
   uint32_t *keys[2], *pos[2];
@@ -894,10 +944,6 @@ int sort_tokens(const Tokens& tk, int64_t n, const Layout& l, char* scratch, con
   const int64_t threads = (n + kClusterThreads - 1) / kClusterThreads;  // full CTAs at one item a thread
   const int most = max_cluster();
   if (threads <= int64_t{most} * kMaxClusterItems) {
-    if (tk.named && tk.vocab > kClusterClears) {
-      const cudaError_t e = cudaMemsetAsync(tk.named, 0, static_cast<size_t>(tk.vocab), st);
-      if (e != cudaSuccess) return failed(e);
-    }
     int ctas = 1, items = 1;
     while (ctas < threads && ctas < most) ctas *= 2;
     while (int64_t{ctas} * items < threads) items *= 2;
@@ -905,12 +951,8 @@ int sort_tokens(const Tokens& tk, int64_t n, const Layout& l, char* scratch, con
                       : items == 2 ? sort_cluster<2>
                       : items == 4 ? sort_cluster<4>
                                    : sort_cluster<kMaxClusterItems>;
-    const cudaError_t e = sort(tk, n, ctas, l.passes, l.digit_bits, keys[0], pos[0], st);
+    const cudaError_t e = sort(tk, n, ctas, l, keys[0], pos[0], st);
     return e == cudaSuccess ? DFC_OK : failed(e);
-  }
-  if (tk.named) {
-    const cudaError_t e = cudaMemsetAsync(tk.named, 0, static_cast<size_t>(tk.vocab), st);
-    if (e != cudaSuccess) return failed(e);
   }
   uint32_t* hist = reinterpret_cast<uint32_t*>(scratch + l.hist);
   const unsigned tiles = static_cast<unsigned>(l.sort_tiles);
@@ -936,20 +978,19 @@ bool sizes_ok(int64_t n, int64_t vocab, int64_t dim) {
 }
 
 template <typename TD, typename TG, bool DROP, bool VEC>
-int run_sums(const SumArgs& s, cudaStream_t st) {
+int run_sums(const SumArgs& s, const Fill& f, cudaStream_t st) {
   const Shape sh = shape(s.dim);
   const int64_t blocks = (s.n + s.block - 1) / s.block;
   const int64_t sum_ctas = blocks * sh.slabs;
-  const int64_t row_bytes = s.dim * static_cast<int64_t>(sizeof(TG));
-  const int rows = static_cast<int>(std::min<int64_t>(kFillRows, std::max<int64_t>(1, 65536 / row_bytes)));
-  const int64_t fill_ctas = s.accumulate ? 0 : (s.vocab + rows - 1) / rows;
+  const int64_t cta_rows = int64_t{f.per_warp} * kSumThreads / 32;
+  const int64_t fill_ctas = f.rows > 0 ? (f.rows + cta_rows - 1) / cta_rows : 0;
   if (sum_ctas + fill_ctas == 0) return DFC_OK;
   cudaError_t e = cudaFuncSetAttribute(sum_kernel<TD, TG, DROP, VEC>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kSumSmem);
   if (e != cudaSuccess) return failed(e);
   e = launch_next(sum_kernel<TD, TG, DROP, VEC>, dim3(static_cast<unsigned>(sum_ctas + fill_ctas)),
                               dim3(sh.lanes, sh.tiles), kSumSmem, st, s, static_cast<uint32_t>(sh.slabs),
-                              static_cast<uint32_t>(sum_ctas), rows);
+                              static_cast<uint32_t>(sum_ctas), f);
   if (e == cudaSuccess && blocks > 1)
     e = launch_next(join_kernel<TG>,
                     dim3(static_cast<unsigned>(blocks - 1),
@@ -959,19 +1000,19 @@ int run_sums(const SumArgs& s, cudaStream_t st) {
 }
 
 template <typename TD, typename TG>
-int by_path(const SumArgs& s, bool drop, cudaStream_t st) {
+int by_path(const SumArgs& s, const Fill& f, bool drop, cudaStream_t st) {
   const bool vec = s.dim % 8 == 0 && aligned(s.dy, 16) && aligned(s.grad, 16) &&
                    s.dy_pitch * static_cast<int64_t>(sizeof(TD)) % 16 == 0 &&
                    s.grad_pitch * static_cast<int64_t>(sizeof(TG)) % 16 == 0;
-  if (vec) return drop ? run_sums<TD, TG, true, true>(s, st) : run_sums<TD, TG, false, true>(s, st);
-  return drop ? run_sums<TD, TG, true, false>(s, st) : run_sums<TD, TG, false, false>(s, st);
+  if (vec) return drop ? run_sums<TD, TG, true, true>(s, f, st) : run_sums<TD, TG, false, true>(s, f, st);
+  return drop ? run_sums<TD, TG, true, false>(s, f, st) : run_sums<TD, TG, false, false>(s, f, st);
 }
 
 template <typename TD>
-int by_grad(const SumArgs& s, int32_t grad_dtype, bool drop, cudaStream_t st) {
-  if (grad_dtype == DFC_DTYPE_F32) return by_path<TD, float>(s, drop, st);
-  if (grad_dtype == DFC_DTYPE_BF16) return by_path<TD, bf16>(s, drop, st);
-  return by_path<TD, f16>(s, drop, st);
+int by_grad(const SumArgs& s, const Fill& f, int32_t grad_dtype, bool drop, cudaStream_t st) {
+  if (grad_dtype == DFC_DTYPE_F32) return by_path<TD, float>(s, f, drop, st);
+  if (grad_dtype == DFC_DTYPE_BF16) return by_path<TD, bf16>(s, f, drop, st);
+  return by_path<TD, f16>(s, f, drop, st);
 }
 
 }  // namespace
@@ -1006,16 +1047,21 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   if (scratch_bytes < l.bytes) return DFC_ERR_SCRATCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* base = static_cast<char*>(scratch);
-  uint8_t* named = accumulate ? nullptr : reinterpret_cast<uint8_t*>(base + l.named);
+  Fill f{};
+  if (!accumulate) {
+    const int64_t size = static_cast<int64_t>(dtype_size(grad_dtype));
+    const uintptr_t all = reinterpret_cast<uintptr_t>(grad) | static_cast<uintptr_t>(grad_pitch * size) |
+                          static_cast<uintptr_t>(dim * size);
+    // about 16 KB a warp
+    const int per_warp = static_cast<int>(std::min<int64_t>(32, std::max<int64_t>(1, 16384 / (dim * size))));
+    f = Fill{static_cast<char*>(grad), grad_pitch * size, dim * size, vocab, per_warp,
+             all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2};
+  }
   if (n_tokens > 0) {
-    const Tokens tk{tokens, token_bytes == 8, vocab, padding_idx, error_flag, named};
+    const Tokens tk{tokens, token_bytes == 8, vocab, padding_idx, error_flag};
     const int rc = sort_tokens(tk, n_tokens, l, base, &s.keys, &s.pos, st);
     if (rc != DFC_OK) return rc;
-  } else if (named && vocab > 0) {
-    const cudaError_t e = cudaMemsetAsync(named, 0, static_cast<size_t>(vocab), st);
-    if (e != cudaSuccess) return failed(e);
   }
-  s.named = named;
   s.n = n_tokens;
   s.tile = l.tile;
   s.block = l.block;
@@ -1033,7 +1079,7 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   s.wide_grad = aligned(grad, 32) && grad_pitch % 8 == 0;
   s.partial = reinterpret_cast<float*>(base + l.partial);
   s.partial_pitch = l.partial_pitch;
-  if (dy_dtype == DFC_DTYPE_F32) return by_grad<float>(s, grad_dtype, drop, st);
-  if (dy_dtype == DFC_DTYPE_BF16) return by_grad<bf16>(s, grad_dtype, drop, st);
-  return by_grad<f16>(s, grad_dtype, drop, st);
+  if (dy_dtype == DFC_DTYPE_F32) return by_grad<float>(s, f, grad_dtype, drop, st);
+  if (dy_dtype == DFC_DTYPE_BF16) return by_grad<bf16>(s, f, grad_dtype, drop, st);
+  return by_grad<f16>(s, f, grad_dtype, drop, st);
 }
