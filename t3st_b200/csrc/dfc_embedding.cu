@@ -5,15 +5,16 @@
 //
 // One thread per eight output elements (one dropout group: out is contiguous,
 // so group g is elements 8g..8g+7 of it).  When a row is a whole number of
-// 16-byte pieces the table is read in such pieces; otherwise element by
-// element, consecutive threads reading consecutive runs of a row.
+// 16-byte pieces the table is read in such pieces; otherwise from the 16-byte
+// blocks around the elements, shifted into place, and element by element where
+// a group spans rows.
 #include "dfc_philox.cuh"
 
 namespace dfc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = 4;  // groups per thread
+constexpr int kGroups = 2;  // groups per thread; with registers for 6 CTAs per SM
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_t t) {
   return wide ? static_cast<const int64_t*>(tokens)[t]
@@ -21,7 +22,7 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 }
 
 template <typename TT, typename TO, bool DROP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 6)
     embed_vec_kernel(const void* tokens, int wide, const TT* table, int64_t pitch, int64_t vocab,
                      uint32_t row_groups, int64_t groups, float scale, TO* out, int wide_table,
                      int wide_out, int32_t* error_flag, DropArgs a) {
@@ -68,19 +69,30 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// i / d for i * d < 2^64, with per_d = ceil(2^64 / d) (0 for d = 1).
+__device__ __forceinline__ int64_t row_of(int64_t i, uint64_t per_d) {
+  return per_d ? static_cast<int64_t>(__umul64hi(static_cast<uint64_t>(i), per_d)) : i;
+}
+
 template <typename TT, typename TO, bool DROP>
 __global__ void __launch_bounds__(kThreads)
     embed_any_kernel(const void* tokens, int wide, const TT* table, int64_t pitch, int64_t vocab,
-                     int64_t dim, int64_t n, float scale, TO* out, int out_aligned,
+                     int64_t dim, uint64_t per_dim, int64_t n, float scale, TO* out, int out_aligned,
                      int32_t* error_flag, DropArgs a) {
   const int64_t g = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (8 * g >= n) return;
-  int64_t t = 8 * g / dim;
+  int64_t t = row_of(8 * g, per_dim);
   int64_t d = 8 * g - t * dim;
   int64_t v = token_at(tokens, wide, t);
   float x[8];
+  const bool one_row = d + 8 <= dim && static_cast<uint64_t>(v) < static_cast<uint64_t>(vocab);
+  if (one_row) {
+    unpack8<TT>(load8_any(table + v * pitch + d, 8, table, table + (vocab - 1) * pitch + dim), x);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], scale);
+  }
+#pragma unroll
+  for (int j = 0; !one_row && j < 8; ++j) {
     x[j] = 0.0f;
     if (8 * g + j < n) {
       if (d == dim) {
@@ -139,7 +151,7 @@ int launch(const EmbedCall& c) {
     const int64_t groups = (n + 7) / 8;
     embed_any_kernel<TT, TO, DROP>
         <<<static_cast<unsigned>((groups + kThreads - 1) / kThreads), kThreads, 0, c.st>>>(
-            c.tokens, c.wide, table, c.pitch, c.vocab, c.dim, n, c.scale, out,
+            c.tokens, c.wide, table, c.pitch, c.vocab, c.dim, c.dim > 1 ? ~0ull / c.dim + 1 : 0ull, n, c.scale, out,
             aligned(out, 16) ? 1 : 0, c.error_flag, c.drop);
   }
   return launch_status();

@@ -395,17 +395,6 @@ struct SumArgs {
   DropArgs drop;
 };
 
-// Columns c .. c + 7 (those below dim) of a row, from `at`, in FP32.
-template <typename T, bool VEC>
-__device__ __forceinline__ void row8(const T* at, int64_t c, int64_t dim, int wide, float (&v)[8]) {
-  if constexpr (VEC) {
-    unpack8<T>(load8(at, wide), v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < dim ? to_f32(at[j]) : 0.0f;
-  }
-}
-
 // The fates of the eight elements e[u] .. e[u] + 7 for two rows.  VEC: e is a
 // multiple of eight, they are one group; otherwise they may reach into the next.
 template <bool VEC>
@@ -433,30 +422,58 @@ struct Fates {
     }
   }
 
-  // v[j] = kept ? v[j] : 0 (the scale is applied to the sum)
-  __device__ __forceinline__ void apply(int u, const DropArgs& a, float (&v)[8]) const {
+  // acc[j] += v[j] where kept (the scale is applied to the sum)
+  __device__ __forceinline__ void add(int u, const DropArgs& a, const float (&v)[8], float (&acc)[8]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (VEC ? kept(w[u], j, a.cmp) : (w[u].x >> j) & 1u) ? v[j] : 0.0f;
+    for (int j = 0; j < 8; ++j)
+      if (VEC ? kept(w[u], j, a.cmp) : (w[u].x >> j) & 1u) acc[j] = __fadd_rn(acc[j], v[j]);
   }
 };
 
+template <typename TG>
+__device__ __forceinline__ void put_one(const SumArgs& s, uint32_t key, int64_t c, float sum) {
+  TG* at = static_cast<TG*>(s.grad) + key * s.grad_pitch + c;
+  float v = __fmul_rn(sum, s.scale);
+  if (s.accumulate) v = __fadd_rn(to_f32(*at), v);
+  *at = from_f32<TG>(v);
+}
+
+__device__ __forceinline__ void store8_shared(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Columns c .. c + 7 of a finished row.  Where rows are no whole 16-byte pieces
+// and a warp has one tile (warp != NULL, 256 floats of shared memory), its
+// lanes exchange columns, so that each store covers 32 neighbouring ones.
 template <typename TG, bool VEC>
-__device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t c, float (&v)[8]) {
-  TG* row = static_cast<TG*>(s.grad) + key * s.grad_pitch;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], s.scale);
-  if (s.accumulate) {
-    float g[8];
-    row8<TG, VEC>(row + c, c, s.dim, s.wide_grad, g);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(g[j], v[j]);
-  }
+__device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t c, const float (&sum)[8],
+                                         float* warp) {
   if constexpr (VEC) {
-    store8(row + c, pack8<TG>(v), s.wide_grad);
+    TG* at = static_cast<TG*>(s.grad) + key * s.grad_pitch + c;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(sum[j], s.scale);
+    if (s.accumulate) {
+      float g[8];
+      unpack8<TG>(load8(at, s.wide_grad), g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(g[j], v[j]);
+    }
+    store8(at, pack8<TG>(v), s.wide_grad);
+  } else if (warp) {
+    const int lane = threadIdx.x & 31;
+    store8_shared(warp + 8 * lane, sum);
+    __syncwarp();
+    const int64_t first = c - 8 * lane + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (first + 32 * j < s.dim) put_one<TG>(s, key, first + 32 * j, warp[32 * j + lane]);
+    __syncwarp();
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c + j < s.dim) row[c + j] = from_f32<TG>(v[j]);
+      if (c + j < s.dim) put_one<TG>(s, key, c + j, sum[j]);
   }
 }
 
@@ -566,15 +583,18 @@ struct Rows {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
   }
 
-  __device__ __forceinline__ void get(int stage, int u, uint32_t pos, float (&v)[8]) const {
+  // Row u of the group; VEC: from its stage.
+  __device__ __forceinline__ Raw8<TD> get(int stage, int u, uint32_t pos) const {
     if constexpr (VEC) {
       Raw8<TD> r;
       const uint32_t at = ring + (stage * N + u) * (8 * sizeof(TD) * kSumThreads);
       shared16(at, r.q[0]);
       if constexpr (sizeof(TD) == 4) shared16(at + 16 * kSumThreads, r.q[1]);
-      unpack8<TD>(r, v);
+      return r;
     } else {
-      row8<TD, false>(dy + pos * s.dy_pitch, c, s.dim, 0, v);
+      const TD* whole = static_cast<const TD*>(s.dy);
+      return load8_any(dy + pos * s.dy_pitch, static_cast<int>(min(s.dim - c, int64_t{8})), whole,
+                       whole + (s.n - 1) * s.dy_pitch + s.dim);
     }
   }
 
@@ -585,19 +605,6 @@ struct Rows {
                  : "memory");
   }
 };
-
-__device__ __forceinline__ void store8_shared(float* p, const float (&v)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-
-template <typename TG>
-__device__ __forceinline__ void put_one(const SumArgs& s, uint32_t key, int64_t c, float sum) {
-  TG* at = static_cast<TG*>(s.grad) + key * s.grad_pitch + c;
-  float v = __fmul_rn(sum, s.scale);
-  if (s.accumulate) v = __fadd_rn(to_f32(*at), v);
-  *at = from_f32<TG>(v);
-}
 
 // What a tile leaves for the sums across tiles: the row its first run adds to
 // (it began before the tile), whether that run goes on behind the tile too, and
@@ -631,7 +638,10 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
   const int64_t hi = min(lo + s.tile, s.n);
   const int tid = threadIdx.y * blockDim.x + threadIdx.x;
   Ends mine{kNoKey, kNoKey, 0};
-  if (lo < hi && c < s.dim) {
+  // (lanes behind the last column stay for the exchange of columns)
+  float* warp = nullptr;
+  if (!VEC && blockDim.x >= 32) warp = reinterpret_cast<float*>(smem + kPartBytes) + 8 * (tid & ~31);
+  if (lo < hi && (c < s.dim || warp)) {
     constexpr int N = kGroup<TD>;
     DropKey k{};
     if (DROP) k = drop_key(s.drop);
@@ -650,6 +660,10 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
       uint32_t key[N], pos[N];
       load_ids<N>(s.keys, i, key);
       if (DROP || !VEC) load_ids<N>(s.pos, i, pos);
+      Raw8<TD> raw[N];
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+        if (!VEC && i + u < hi && key[u] < s.vocab && c < s.dim) raw[u] = rows.get(stage, u, pos[u]);
 #pragma unroll
       for (int u = 0; u < N; u += 2) {
         Fates<VEC> fates;
@@ -658,25 +672,28 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
         for (int h = 0; h < 2; ++h) {
           const uint32_t id = key[u + h];
           if (i + u + h >= hi || id >= s.vocab) continue;
+          if (VEC) raw[u + h] = rows.get(stage, u + h, pos[u + h]);
           float v[8];
-          rows.get(stage, u + h, pos[u + h], v);
-          if (DROP) fates.apply(h, s.drop, v);
-          if (id == run) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] = __fadd_rn(acc[j], v[j]);
-          } else {
+          unpack8<TD>(raw[u + h], v);
+          if (id != run) {
             if (run != kNoKey) {
               if (first && run == before) {
                 store8_shared(part + 8 * tid, acc);
                 mine.head = run;
               } else {
-                put_row8<TG, VEC>(s, run, c, acc);
+                put_row8<TG, VEC>(s, run, c, acc, warp);
               }
               first = false;
             }
             run = id;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] = v[j];
+            for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+          }
+          if (DROP) {
+            fates.add(h, s.drop, v, acc);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] = __fadd_rn(acc[j], v[j]);
           }
         }
       }
@@ -692,7 +709,7 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
         store8_shared(part + 8 * (kSumThreads + tid), acc);
         mine.tail = run;
       } else {
-        put_row8<TG, VEC>(s, run, c, acc);
+        put_row8<TG, VEC>(s, run, c, acc, warp);
       }
     }
   }

@@ -269,6 +269,43 @@ __device__ __forceinline__ void store8(T* p, const Raw8<T>& r, int wide) {
   q[0] = r.q[0];
 }
 
+// Eight elements from any address, p aligned to T, of an array that occupies
+// [lo, hi): the 16-byte blocks around them and a shift, where the blocks lie
+// within the array, otherwise element by element.  `count` of them are needed;
+// what the others hold is undefined.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8_any(const T* p, int count, const void* lo, const void* hi) {
+  constexpr int kBlocks = sizeof(T) / 2 + 1;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), first = at & ~uintptr_t{15};
+  const uint32_t off = static_cast<uint32_t>(at & 15);
+  Raw8<T> r;
+  if (first >= reinterpret_cast<uintptr_t>(lo) && first + 16 * kBlocks <= reinterpret_cast<uintptr_t>(hi)) {
+    uint32_t w[4 * kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const uint4 q = reinterpret_cast<const uint4*>(first)[b];
+      w[4 * b] = q.x, w[4 * b + 1] = q.y, w[4 * b + 2] = q.z, w[4 * b + 3] = q.w;
+    }
+    // down by off bytes: two words, one word, half a word
+#pragma unroll
+    for (int i = 0; i < 4 * kBlocks - 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4 * kBlocks - 3; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], off & 2 ? 16 : 0);
+    }
+#pragma unroll
+    for (int b = 0; b < kBlocks - 1; ++b) r.q[b] = make_uint4(w[4 * b], w[4 * b + 1], w[4 * b + 2], w[4 * b + 3]);
+    return r;
+  }
+  T v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < count ? p[j] : T(0.0f);
+  memcpy(&r, v, sizeof(r));
+  return r;
+}
+
 inline bool known_dtype(int32_t d) {
   return d == DFC_DTYPE_F32 || d == DFC_DTYPE_BF16 || d == DFC_DTYPE_F16;
 }
