@@ -12,6 +12,8 @@
 //      in the scratch.  More CTAs of the same grid zero the rows of an
 //      overwritten grad that no token names;
 //   3. join_kernel adds such a run's partial rows in a fixed order.
+// Up to kSmallTokens, step 1 is left out: every CTA of the sums sorts the
+// tokens for itself.
 // No atomics on floats: the same inputs give the same bits.
 #include <cooperative_groups.h>
 
@@ -390,6 +392,8 @@ struct SumArgs {
   int accumulate;
   int wide_dy, wide_grad;  // rows on 32-byte boundaries
   int64_t block;         // positions of a CTA's tiles
+  Tokens tokens;         // SMALL: sorted by every CTA; the first one writes `keys` out for the join
+  uint32_t* keys_out;
   float* partial;        // 2 rows a block: a run from before it, a run that goes on behind it
   int64_t partial_pitch; // dim rounded up to 8
   DropArgs drop;
@@ -551,6 +555,7 @@ template <typename TD, typename TG, bool VEC>
 struct Rows {
   static constexpr int N = kGroup<TD>;
   const SumArgs& s;
+  const uint32_t *keys, *ids;  // sorted, with their positions
   const TD* dy;  // column c of row 0
   int64_t c, hi;
   uint32_t ring;  // this thread's slot of the first stage
@@ -560,8 +565,8 @@ struct Rows {
   __device__ __forceinline__ void request(int64_t i, int stage) const {
     if (VEC && i < hi) {
       uint32_t key[N], pos[N];
-      load_ids<N>(s.keys, i, key);
-      load_ids<N>(s.pos, i, pos);
+      load_ids<N>(keys, i, key);
+      load_ids<N>(ids, i, pos);
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         if (i + u < hi && key[u] < s.vocab) {
@@ -616,10 +621,107 @@ struct Ends {
 constexpr int kSumSmem = kPartBytes + kRingBytes + static_cast<int>(sizeof(Ends)) * kSumThreads;
 constexpr int kSumCtas = 3;  // per SM
 
+// ---- up to kSmallTokens tokens: one CTA sorts them alone -----------------------
+constexpr int kSmallTokens = 4 * kSumThreads;
+constexpr int kSmallBits = 10;  // of a position
+constexpr int64_t kSmallVocab = int64_t{1} << (32 - kSmallBits);
+
+__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b, bool up) {
+  const uint32_t lo = min(a, b), hi = max(a, b);
+  a = up ? lo : hi;
+  b = up ? hi : lo;
+}
+
+// Bitonic sort of kSumThreads * E words key << 10 | position, E consecutive
+// ones a thread: distances within a thread in registers, within a warp by
+// shuffles, the others through `words` in shared memory.  All words differ
+// (padding aside), so the order is by key, then position.
+template <int E>
+__device__ __noinline__ void small_sort(uint32_t (&x)[4], uint32_t* words, int tid) {
+#pragma unroll 1
+  for (int k = 2; k <= kSumThreads * E; k <<= 1) {
+#pragma unroll 1
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (j < E) {
+        if (E >= 2 && j == 1) {
+          exchange(x[0], x[1], (tid * E & k) == 0);
+          if (E == 4) exchange(x[2], x[3], (tid * E + 2 & k) == 0);
+        } else if (E == 4) {
+          exchange(x[0], x[2], (tid * E & k) == 0);
+          exchange(x[1], x[3], (tid * E & k) == 0);
+        }
+        continue;
+      }
+      if (j >= 32 * E) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) words[tid * E + e] = x[e];
+        __syncthreads();
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = tid * E + e;
+        const uint32_t y = j >= 32 * E ? words[i ^ j] : __shfl_xor_sync(0xFFFFFFFFu, x[e], j / E);
+        x[e] = ((i & j) == 0) == ((i & k) == 0) ? min(x[e], y) : max(x[e], y);
+      }
+    }
+  }
+}
+
+// keys[i], pos[i] of the n tokens in sorted order, in shared memory (whole groups
+// of four: read, not used, behind n).
+__device__ __forceinline__ void small_sort_tokens(const Tokens& tk, int n, uint32_t* keys, uint32_t* pos) {
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const int e = n <= kSumThreads ? 1 : n <= 2 * kSumThreads ? 2 : 4;  // items a thread
+  uint32_t x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int t = tid * e + j;
+    x[j] = j < e && t < n ? token_key(tk, t) << kSmallBits | t : 0xFFFFFFFFu;
+  }
+  if (e == 1)
+    small_sort<1>(x, keys, tid);
+  else if (e == 2)
+    small_sort<2>(x, keys, tid);
+  else
+    small_sort<4>(x, keys, tid);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j < e) {
+      keys[tid * e + j] = x[j] >> kSmallBits;
+      pos[tid * e + j] = x[j] & ((1u << kSmallBits) - 1);
+    }
+  }
+  __syncthreads();
+}
+
+// fill_searched() without sorted keys: the CTA looks at all tokens.
+__device__ __forceinline__ void fill_marked(const Tokens& tk, int n, const Fill& f, uint32_t cta, void* zeros,
+                                            uint32_t* named) {
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, warp = tid >> 5;
+  const int64_t first = static_cast<int64_t>(cta) * (kSumThreads / 32) * f.per_warp;
+  clear_zeros(zeros);
+  if (tid < kSumThreads / 32) named[tid] = 0u;  // one word a warp, a bit per row
+  __syncthreads();
+  for (int t = tid; t < n; t += kSumThreads) {
+    const uint32_t row = token_key(tk, t) - static_cast<uint32_t>(first);
+    const uint32_t owner = row / f.per_warp;
+    if (owner < kSumThreads / 32) atomicOr(&named[owner], 1u << (row % f.per_warp));
+  }
+  __syncthreads();
+  const int64_t mine = first + static_cast<int64_t>(warp) * f.per_warp, left = f.rows - mine;
+  uint32_t empty = ~named[warp];
+  const int64_t rows = min(left, static_cast<int64_t>(f.per_warp));
+  if (rows < 32) empty &= rows > 0 ? (1u << rows) - 1 : 0u;
+  fill_rows(f, mine, empty, zeros);
+  fill_done();
+}
+
 // A CTA sums blockDim.y tiles, one after the other, of a slab of 8 * blockDim.x
 // columns; those behind sum_ctas zero rows (in the order of their addresses:
 // spread evenly among the others they took 460 us instead of 420 in all).
-template <typename TD, typename TG, bool DROP, bool VEC>
+template <typename TD, typename TG, bool DROP, bool VEC, bool SMALL>
 __global__ void __launch_bounds__(kSumThreads, kSumCtas)
     sum_kernel(SumArgs s, uint32_t slabs, uint32_t sum_ctas, Fill f) {
   extern __shared__ __align__(128) unsigned char smem[];  // kSumSmem bytes
@@ -627,9 +729,20 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
   Ends* ends = reinterpret_cast<Ends*>(smem + kPartBytes + kRingBytes);
   let_next_start();
   wait_for_previous();
+  uint32_t* small = reinterpret_cast<uint32_t*>(smem + kSumSmem);  // SMALL: 2 * kSmallTokens words
   if (blockIdx.x >= sum_ctas) {
-    fill_searched(s, f, blockIdx.x - sum_ctas, smem);
+    if (SMALL)
+      fill_marked(s.tokens, static_cast<int>(s.n), f, blockIdx.x - sum_ctas, smem, small);
+    else
+      fill_searched(s, f, blockIdx.x - sum_ctas, smem);
     return;
+  }
+  const uint32_t* keys = SMALL ? small : s.keys;
+  const uint32_t* ids = SMALL ? small + kSmallTokens : s.pos;
+  if (SMALL) {
+    small_sort_tokens(s.tokens, static_cast<int>(s.n), small, small + kSmallTokens);
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < s.n; i += kSumThreads) s.keys_out[i] = keys[i];
   }
   const int64_t block = blockIdx.x / slabs;
   const int64_t c0 = 8ll * (blockIdx.x % slabs) * blockDim.x;
@@ -645,10 +758,10 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
     constexpr int N = kGroup<TD>;
     DropKey k{};
     if (DROP) k = drop_key(s.drop);
-    const Rows<TD, TG, VEC> rows{s, static_cast<const TD*>(s.dy) + c, c, hi,
+    const Rows<TD, TG, VEC> rows{s, keys, ids, static_cast<const TD*>(s.dy) + c, c, hi,
                                  static_cast<uint32_t>(__cvta_generic_to_shared(smem + kPartBytes)) + 16 * tid};
-    const uint32_t before = lo > 0 ? s.keys[lo - 1] : kNoKey;
-    const uint32_t behind = hi < s.n ? s.keys[hi] : kNoKey;
+    const uint32_t before = lo > 0 ? keys[lo - 1] : kNoKey;
+    const uint32_t behind = hi < s.n ? keys[hi] : kNoKey;
     float acc[8];
     uint32_t run = kNoKey;
     bool first = true;  // no run of the tile has ended yet
@@ -658,8 +771,8 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
     for (int64_t i = lo; i < hi; i += N) {
       rows.arrived();
       uint32_t key[N], pos[N];
-      load_ids<N>(s.keys, i, key);
-      if (DROP || !VEC) load_ids<N>(s.pos, i, pos);
+      load_ids<N>(keys, i, key);
+      if (DROP || !VEC) load_ids<N>(ids, i, pos);
       Raw8<TD> raw[N];
 #pragma unroll
       for (int u = 0; u < N; ++u)
@@ -994,26 +1107,36 @@ bool sizes_ok(int64_t n, int64_t vocab, int64_t dim) {
          dim <= DFC_MAX_DIM && n * dim <= (int64_t{1} << 39);
 }
 
-template <typename TD, typename TG, bool DROP, bool VEC>
-int run_sums(const SumArgs& s, const Fill& f, cudaStream_t st) {
+template <typename TD, typename TG, bool DROP, bool VEC, bool SMALL>
+int launch_sums(const SumArgs& s, const Fill& f, cudaStream_t st) {
   const Shape sh = shape(s.dim);
   const int64_t blocks = (s.n + s.block - 1) / s.block;
   const int64_t sum_ctas = blocks * sh.slabs;
   const int64_t cta_rows = int64_t{f.per_warp} * kSumThreads / 32;
   const int64_t fill_ctas = f.rows > 0 ? (f.rows + cta_rows - 1) / cta_rows : 0;
   if (sum_ctas + fill_ctas == 0) return DFC_OK;
-  cudaError_t e = cudaFuncSetAttribute(sum_kernel<TD, TG, DROP, VEC>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSumSmem);
+  const auto kernel = sum_kernel<TD, TG, DROP, VEC, SMALL>;
+  const int smem = kSumSmem + (SMALL ? 8 * kSmallTokens : 0);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return failed(e);
-  e = launch_next(sum_kernel<TD, TG, DROP, VEC>, dim3(static_cast<unsigned>(sum_ctas + fill_ctas)),
-                              dim3(sh.lanes, sh.tiles), kSumSmem, st, s, static_cast<uint32_t>(sh.slabs),
-                              static_cast<uint32_t>(sum_ctas), f);
+  e = launch_next(kernel, dim3(static_cast<unsigned>(sum_ctas + fill_ctas)), dim3(sh.lanes, sh.tiles), smem, st,
+                  s, static_cast<uint32_t>(sh.slabs), static_cast<uint32_t>(sum_ctas), f);
   if (e == cudaSuccess && blocks > 1)
     e = launch_next(join_kernel<TG>,
                     dim3(static_cast<unsigned>(blocks - 1),
                          static_cast<unsigned>((s.dim + 4 * kJoinLanes - 1) / (4 * kJoinLanes))),
                     dim3(kJoinLanes, kJoinParts), 0, st, s);
   return e == cudaSuccess ? launch_status() : failed(e);
+}
+
+// Every CTA sorts the tokens itself: one launch less, 17.2 -> 14.2 us for 300
+// tokens of 384 FP32 columns.
+bool small(int64_t n, int64_t vocab) { return n <= kSmallTokens && vocab < kSmallVocab; }
+
+template <typename TD, typename TG, bool DROP, bool VEC>
+int run_sums(const SumArgs& s, const Fill& f, cudaStream_t st) {
+  return small(s.n, s.vocab) ? launch_sums<TD, TG, DROP, VEC, true>(s, f, st)
+                             : launch_sums<TD, TG, DROP, VEC, false>(s, f, st);
 }
 
 template <typename TD, typename TG>
@@ -1074,9 +1197,11 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
     f = Fill{static_cast<char*>(grad), grad_pitch * size, dim * size, vocab, per_warp,
              all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2};
   }
-  if (n_tokens > 0) {
-    const Tokens tk{tokens, token_bytes == 8, vocab, padding_idx, error_flag};
-    const int rc = sort_tokens(tk, n_tokens, l, base, &s.keys, &s.pos, st);
+  s.tokens = Tokens{tokens, token_bytes == 8, vocab, padding_idx, error_flag};
+  s.keys_out = reinterpret_cast<uint32_t*>(base + l.keys[0]);
+  s.keys = s.keys_out;
+  if (n_tokens > 0 && !small(n_tokens, vocab)) {
+    const int rc = sort_tokens(s.tokens, n_tokens, l, base, &s.keys, &s.pos, st);
     if (rc != DFC_OK) return rc;
   }
   s.n = n_tokens;
