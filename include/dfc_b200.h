@@ -187,6 +187,7 @@ typedef struct DfcDropout {
 #define DFC_MAX_TOKENS (INT64_C(1) << 28)
 #define DFC_MAX_VOCAB (INT64_C(1) << 30)
 #define DFC_MAX_DIM (INT64_C(1) << 20)
+#define DFC_MAX_PITCH INT64_C(0x7FFFFFFF) /* elements from row to row */
 
 DFC_API int dfc_abi_version(void);
 DFC_API const char* dfc_strerror(int status);

@@ -23,7 +23,7 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 
 template <typename TT, typename TO, bool DROP>
 __global__ void __launch_bounds__(kThreads, 6)
-    embed_vec_kernel(const void* tokens, int wide, const TT* table, int64_t pitch, int64_t vocab,
+    embed_vec_kernel(const void* tokens, int wide, const TT* table, uint32_t pitch, int64_t vocab,
                      uint32_t row_groups, int64_t groups, float scale, TO* out, int wide_table,
                      int wide_out, int32_t* error_flag, DropArgs a) {
   const int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads * kGroups);
@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(kThreads, 6)
       const uint32_t dt = q / row_groups;
       const int64_t v = token_at(tokens, wide, t0 + dt);
       bad[u] = static_cast<uint64_t>(v) >= static_cast<uint64_t>(vocab);
-      if (!bad[u]) X[u] = load8(table + v * pitch + 8ll * (q - dt * row_groups), wide_table);
+      if (!bad[u]) X[u] = load8(table + static_cast<uint64_t>(static_cast<uint32_t>(v)) * pitch + 8ll * (q - dt * row_groups), wide_table);
     }
   }
   uint4 w[kGroups];
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads)
   float x[8];
   const bool one_row = d + 8 <= dim && static_cast<uint64_t>(v) < static_cast<uint64_t>(vocab);
   if (one_row) {
-    unpack8<TT>(load8_any(table + v * pitch + d, 8, table, table + (vocab - 1) * pitch + dim), x);
+    unpack8<TT>(load8_any(table + v * pitch + d, table, table + (vocab - 1) * pitch + dim), x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], scale);
   }
@@ -145,7 +145,7 @@ int launch(const EmbedCall& c) {
   if (vec) {
     const int64_t groups = n / 8, tile = kThreads * kGroups;
     embed_vec_kernel<TT, TO, DROP><<<static_cast<unsigned>((groups + tile - 1) / tile), kThreads, 0, c.st>>>(
-        c.tokens, c.wide, table, c.pitch, c.vocab, static_cast<uint32_t>(c.dim / 8), groups, c.scale,
+        c.tokens, c.wide, table, static_cast<uint32_t>(c.pitch), c.vocab, static_cast<uint32_t>(c.dim / 8), groups, c.scale,
         out, aligned(table, 32) && c.pitch % 8 == 0, aligned(out, 32), c.error_flag, c.drop);
   } else {
     const int64_t groups = (n + 7) / 8;
@@ -173,7 +173,7 @@ extern "C" int dfc_embedding(const void* tokens, int32_t token_bytes, int64_t n_
                              const DfcDropout* dropout, int32_t* error_flag, void* stream) {
   using namespace dfc;
   if (n_tokens < 0 || n_tokens > DFC_MAX_TOKENS || vocab < 0 || vocab > DFC_MAX_VOCAB || dim < 0 ||
-      dim > DFC_MAX_DIM || table_pitch < 0 || n_tokens * dim > (int64_t{1} << 39))
+      dim > DFC_MAX_DIM || table_pitch < 0 || table_pitch > DFC_MAX_PITCH || n_tokens * dim > (int64_t{1} << 39))
     return DFC_ERR_SIZE;
   if ((token_bytes != 4 && token_bytes != 8) || !known_dtype(table_dtype) || !known_dtype(out_dtype))
     return DFC_ERR_DTYPE;

@@ -378,26 +378,33 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
 }
 
 // ---- 2. sums of runs ------------------------------------------------------------
+// Everything but addresses fits 32 bits: a row's place is one 32 x 32 -> 64-bit
+// product.
 struct SumArgs {
   const uint32_t* keys;  // sorted
   const uint32_t* pos;
-  int64_t n;
-  int tile;              // K
+  uint32_t n;
+  uint32_t tile;         // K
+  uint32_t block;        // positions of a CTA's tiles
   const void* dy;
-  int64_t dy_pitch;
+  uint32_t dy_pitch;
   void* grad;
-  int64_t grad_pitch;
-  int64_t vocab, dim;
+  uint32_t grad_pitch;
+  uint32_t vocab, dim;
   float scale;
   int accumulate;
   int wide_dy, wide_grad;  // rows on 32-byte boundaries
-  int64_t block;         // positions of a CTA's tiles
   Tokens tokens;         // SMALL: sorted by every CTA; the first one writes `keys` out for the join
   uint32_t* keys_out;
   float* partial;        // 2 rows a block: a run from before it, a run that goes on behind it
-  int64_t partial_pitch; // dim rounded up to 8
+  uint32_t partial_pitch;  // dim rounded up to 8
   DropArgs drop;
 };
+
+template <typename T>
+__device__ __forceinline__ T* row_at(T* base, uint32_t row, uint32_t pitch) {
+  return base + static_cast<uint64_t>(row) * pitch;
+}
 
 // The fates of the eight elements e[u] .. e[u] + 7 for two rows.  VEC: e is a
 // multiple of eight, they are one group; otherwise they may reach into the next.
@@ -405,8 +412,8 @@ template <bool VEC>
 struct Fates {
   uint4 w[2];
 
-  __device__ __forceinline__ void set(const int64_t (&e)[2], const DropArgs& a, const DropKey& k) {
-    uint64_t g[2] = {static_cast<uint64_t>(e[0]) >> 3, static_cast<uint64_t>(e[1]) >> 3};
+  __device__ __forceinline__ void set(const uint64_t (&e)[2], const DropArgs& a, const DropKey& k) {
+    uint64_t g[2] = {e[0] >> 3, e[1] >> 3};
     drop_words<2>(g, a, k, w);
     if constexpr (!VEC) {  // w[u].x: one bit per element
       uint32_t bits[2] = {0u, 0u};
@@ -435,8 +442,8 @@ struct Fates {
 };
 
 template <typename TG>
-__device__ __forceinline__ void put_one(const SumArgs& s, uint32_t key, int64_t c, float sum) {
-  TG* at = static_cast<TG*>(s.grad) + key * s.grad_pitch + c;
+__device__ __forceinline__ void put_one(const SumArgs& s, uint32_t key, uint32_t c, float sum) {
+  TG* at = row_at(static_cast<TG*>(s.grad), key, s.grad_pitch) + c;
   float v = __fmul_rn(sum, s.scale);
   if (s.accumulate) v = __fadd_rn(to_f32(*at), v);
   *at = from_f32<TG>(v);
@@ -451,10 +458,10 @@ __device__ __forceinline__ void store8_shared(float* p, const float (&v)[8]) {
 // and a warp has one tile (warp != NULL, 256 floats of shared memory), its
 // lanes exchange columns, so that each store covers 32 neighbouring ones.
 template <typename TG, bool VEC>
-__device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t c, const float (&sum)[8],
+__device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, uint32_t c, const float (&sum)[8],
                                          float* warp) {
   if constexpr (VEC) {
-    TG* at = static_cast<TG*>(s.grad) + key * s.grad_pitch + c;
+    TG* at = row_at(static_cast<TG*>(s.grad), key, s.grad_pitch) + c;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(sum[j], s.scale);
@@ -469,10 +476,16 @@ __device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t
     const int lane = threadIdx.x & 31;
     store8_shared(warp + 8 * lane, sum);
     __syncwarp();
-    const int64_t first = c - 8 * lane + lane;
+    const int first = static_cast<int>(c) - 7 * lane, left = static_cast<int>(s.dim) - first;
+    TG* at = row_at(static_cast<TG*>(s.grad), key, s.grad_pitch) + first;
+    float g[8];  // all loads before the first store
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (first + 32 * j < s.dim) put_one<TG>(s, key, first + 32 * j, warp[32 * j + lane]);
+    for (int j = 0; j < 8; ++j) g[j] = s.accumulate && 32 * j < left ? to_f32(at[32 * j]) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = __fmul_rn(warp[32 * j + lane], s.scale);
+      if (32 * j < left) at[32 * j] = from_f32<TG>(s.accumulate ? __fadd_rn(g[j], v) : v);
+    }
     __syncwarp();
   } else {
 #pragma unroll
@@ -483,27 +496,31 @@ __device__ __forceinline__ void put_row8(const SumArgs& s, uint32_t key, int64_t
 
 constexpr int kSumThreads = 256;
 constexpr int kSumLanes = 64;  // threads of a tile's slab of 512 columns, at most
-// Rows that a thread has on the way: kStages groups of kGroup<T> 16-byte or
-// 32-byte pieces, in shared memory of its own.
+// Rows that a thread has on the way, in shared memory of its own: kStages groups
+// of `rows` rows, `pieces` 16-byte pieces each (whole ones, or the blocks around
+// eight elements that lie anywhere).
 constexpr int kStages = 2;
-template <typename TD>
-constexpr int kGroup = sizeof(TD) == 2 ? 4 : 2;
-constexpr int kRingBytes = kStages * 4 * 16 * kSumThreads;
+template <typename TD, bool VEC>
+struct Ring {
+  static constexpr int pieces = VEC ? sizeof(TD) / 2 : Blocks<TD>::N;
+  static constexpr int rows = VEC && sizeof(TD) == 2 ? 4 : 2;
+  static constexpr int bytes = kStages * rows * pieces * 16 * kSumThreads;
+};
 constexpr int kPartBytes = 2 * 8 * 4 * kSumThreads;
-static_assert(kPartBytes >= kZeroBytes, "fill_ranges() keeps its zeros there");
+static_assert(kPartBytes >= kZeroBytes, "the zeros that rows are filled from lie there");
 
 // The first position at which the sorted keys reach `row` (lanes 0..15 of the
 // warp) or `end` (lanes 16..31): each step, the half-warp's lanes look at the 16
 // ends of equal parts of what is left.
-__device__ __forceinline__ int64_t half_warp_search(const SumArgs& s, int64_t row) {
+__device__ __forceinline__ uint32_t half_warp_search(const SumArgs& s, uint32_t row) {
   const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31;
-  int64_t a = 0, b = s.n;  // keys before a are below row, keys from b on are not
+  uint32_t a = 0, b = s.n;  // keys before a are below row, keys from b on are not
   while (__any_sync(0xFFFFFFFFu, a < b)) {
-    const int64_t step = (b - a + 15) / 16, at = a + ((lane & 15) + 1) * step - 1;
+    const uint32_t step = (b - a + 15) / 16, at = a + ((lane & 15) + 1) * step - 1;
     const bool below = a < b && at < b && s.keys[at] < row;  // one half may be done before the other
     const int parts = __popc((__ballot_sync(0xFFFFFFFFu, below) >> (lane & 16)) & 0xFFFFu);
     if (a < b) {
-      const int64_t next = a + parts * step;
+      const uint32_t next = a + parts * step;
       b = min(b, next + step - 1);
       a = min(next, b);
     }
@@ -515,16 +532,16 @@ __device__ __forceinline__ int64_t half_warp_search(const SumArgs& s, int64_t ro
 __device__ __forceinline__ void fill_searched(const SumArgs& s, const Fill& f, uint32_t cta, void* zeros) {
   clear_zeros(zeros);
   const int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid & 31;
-  const int64_t first = (static_cast<int64_t>(cta) * (kSumThreads / 32) + (tid >> 5)) * f.per_warp;
-  const int64_t found = half_warp_search(s, lane < 16 ? first : first + f.per_warp);
-  int64_t a = __shfl_sync(0xFFFFFFFFu, found, 0);
-  const int64_t end = __shfl_sync(0xFFFFFFFFu, found, 16);
-  const int64_t row = first + lane;
+  const uint32_t first = (cta * (kSumThreads / 32) + (tid >> 5)) * f.per_warp;  // rows < 2^30 + a CTA's
+  const uint32_t found = half_warp_search(s, lane < 16 ? first : first + f.per_warp);
+  uint32_t a = __shfl_sync(0xFFFFFFFFu, found, 0);
+  const uint32_t end = __shfl_sync(0xFFFFFFFFu, found, 16);
+  const uint32_t row = first + lane;
   bool empty = false;
   if (lane < f.per_warp && row < f.rows) {
-    int64_t b = end;  // the first key >= row lies in [a, end]
+    uint32_t b = end;  // the first key >= row lies in [a, end]
     while (a < b) {
-      const int64_t m = (a + b) / 2;
+      const uint32_t m = (a + b) / 2;
       if (s.keys[m] < row)
         a = m + 1;
       else
@@ -540,7 +557,7 @@ __device__ __forceinline__ void fill_searched(const SumArgs& s, const Fill& f, u
 // N keys from position i on (kNoKey behind hi); i is a multiple of N and the
 // arrays are allocated in whole tiles.
 template <int N>
-__device__ __forceinline__ void load_ids(const uint32_t* ids, int64_t i, uint32_t (&v)[N]) {
+__device__ __forceinline__ void load_ids(const uint32_t* ids, uint32_t i, uint32_t (&v)[N]) {
   if constexpr (N == 4) {
     const uint4 q = *reinterpret_cast<const uint4*>(ids + i);
     v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
@@ -553,31 +570,44 @@ __device__ __forceinline__ void load_ids(const uint32_t* ids, int64_t i, uint32_
 // The rows of a tile, columns c .. c + 7, group by group.
 template <typename TD, typename TG, bool VEC>
 struct Rows {
-  static constexpr int N = kGroup<TD>;
+  static constexpr int N = Ring<TD, VEC>::rows, P = Ring<TD, VEC>::pieces;
   const SumArgs& s;
   const uint32_t *keys, *ids;  // sorted, with their positions
-  const TD* dy;  // column c of row 0
-  int64_t c, hi;
-  uint32_t ring;  // this thread's slot of the first stage
+  const TD* dy;                // column c of row 0
+  uint32_t c, hi;
+  uint32_t ring;               // this thread's slot of the first piece
+
+  __device__ __forceinline__ uint32_t slot(int stage, int u, int p) const {
+    return ring + ((stage * N + u) * P + p) * (16 * kSumThreads);
+  }
+
+  // Whole pieces, or blocks that lie within dy.
+  __device__ __forceinline__ bool by_pieces(const TD* from) const {
+    if (VEC) return true;
+    const TD* whole = static_cast<const TD*>(s.dy);
+    return Blocks<TD>::within(from, whole, row_at(whole, s.n - 1, s.dy_pitch) + s.dim);
+  }
 
   // Rows of the group at i go on their way into stage `stage`.  Rows of an
   // accumulated grad that the ends of its runs will read are brought into L2.
-  __device__ __forceinline__ void request(int64_t i, int stage) const {
-    if (VEC && i < hi) {
+  __device__ __forceinline__ void request(uint32_t i, int stage) const {
+    if (i < hi && c < s.dim) {
       uint32_t key[N], pos[N];
       load_ids<N>(keys, i, key);
       load_ids<N>(ids, i, pos);
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         if (i + u < hi && key[u] < s.vocab) {
-          const TD* from = dy + pos[u] * s.dy_pitch;
-          const uint32_t to = ring + (stage * N + u) * (8 * sizeof(TD) * kSumThreads);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-          if constexpr (sizeof(TD) == 4)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * kSumThreads), "l"(from + 4)
-                         : "memory");
+          const TD* from = row_at(dy, pos[u], s.dy_pitch);
+          if (by_pieces(from)) {
+            const char* piece = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t{15});
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(stage, u, p)), "l"(piece + 16 * p)
+                           : "memory");
+          }
           if (s.accumulate && (u == 0 || key[u] != key[u - 1]))
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const TG*>(s.grad) + key[u] * s.grad_pitch + c));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(row_at(static_cast<const TG*>(s.grad), key[u], s.grad_pitch) + c));
         }
       }
     }
@@ -588,18 +618,20 @@ struct Rows {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
   }
 
-  // Row u of the group; VEC: from its stage.
+  // Row u of the group; what lies behind the last column is undefined.
   __device__ __forceinline__ Raw8<TD> get(int stage, int u, uint32_t pos) const {
     if constexpr (VEC) {
       Raw8<TD> r;
-      const uint32_t at = ring + (stage * N + u) * (8 * sizeof(TD) * kSumThreads);
-      shared16(at, r.q[0]);
-      if constexpr (sizeof(TD) == 4) shared16(at + 16 * kSumThreads, r.q[1]);
+#pragma unroll
+      for (int p = 0; p < P; ++p) shared16(slot(stage, u, p), r.q[p]);
       return r;
     } else {
-      const TD* whole = static_cast<const TD*>(s.dy);
-      return load8_any(dy + pos * s.dy_pitch, static_cast<int>(min(s.dim - c, int64_t{8})), whole,
-                       whole + (s.n - 1) * s.dy_pitch + s.dim);
+      const TD* from = row_at(dy, pos, s.dy_pitch);
+      if (!by_pieces(from)) return load8_single(from, static_cast<int>(min(s.dim - c, 8u)));
+      Blocks<TD> b;
+#pragma unroll
+      for (int p = 0; p < P; ++p) shared16(slot(stage, u, p), b.q[p]);
+      return b.at(from);
     }
   }
 
@@ -618,7 +650,16 @@ struct Ends {
   uint32_t head, tail;  // kNoKey: none
   int through;
 };
-constexpr int kSumSmem = kPartBytes + kRingBytes + static_cast<int>(sizeof(Ends)) * kSumThreads;
+constexpr int kEndsBytes = static_cast<int>(sizeof(Ends)) * kSumThreads;
+constexpr int kExchangeBytes = 8 * 4 * kSumThreads;  // put_row8()
+// Shared memory: part | ends | exchange (rows of any width) | sorted tokens (SMALL) | ring
+template <typename TD, bool VEC, bool SMALL>
+struct SumSmem {
+  static constexpr int exchange = kPartBytes + kEndsBytes;
+  static constexpr int tokens = exchange + (VEC ? 0 : kExchangeBytes);
+  static constexpr int ring = tokens + (SMALL ? 8 * 4 * kSumThreads : 0);
+  static constexpr int bytes = ring + Ring<TD, VEC>::bytes;
+};
 constexpr int kSumCtas = 3;  // per SM
 
 // ---- up to kSmallTokens tokens: one CTA sorts them alone -----------------------
@@ -724,12 +765,13 @@ __device__ __forceinline__ void fill_marked(const Tokens& tk, int n, const Fill&
 template <typename TD, typename TG, bool DROP, bool VEC, bool SMALL>
 __global__ void __launch_bounds__(kSumThreads, kSumCtas)
     sum_kernel(SumArgs s, uint32_t slabs, uint32_t sum_ctas, Fill f) {
-  extern __shared__ __align__(128) unsigned char smem[];  // kSumSmem bytes
+  using Smem = SumSmem<TD, VEC, SMALL>;
+  extern __shared__ __align__(128) unsigned char smem[];  // Smem::bytes
   float* part = reinterpret_cast<float*>(smem);            // [head, tail][tile][column]
-  Ends* ends = reinterpret_cast<Ends*>(smem + kPartBytes + kRingBytes);
+  Ends* ends = reinterpret_cast<Ends*>(smem + kPartBytes);
   let_next_start();
   wait_for_previous();
-  uint32_t* small = reinterpret_cast<uint32_t*>(smem + kSumSmem);  // SMALL: 2 * kSmallTokens words
+  uint32_t* small = reinterpret_cast<uint32_t*>(smem + Smem::tokens);  // SMALL: 2 * kSmallTokens words
   if (blockIdx.x >= sum_ctas) {
     if (SMALL)
       fill_marked(s.tokens, static_cast<int>(s.n), f, blockIdx.x - sum_ctas, smem, small);
@@ -742,24 +784,24 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
   if (SMALL) {
     small_sort_tokens(s.tokens, static_cast<int>(s.n), small, small + kSmallTokens);
     if (blockIdx.x == 0)
-      for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < s.n; i += kSumThreads) s.keys_out[i] = keys[i];
+      for (uint32_t i = threadIdx.y * blockDim.x + threadIdx.x; i < s.n; i += kSumThreads) s.keys_out[i] = keys[i];
   }
-  const int64_t block = blockIdx.x / slabs;
-  const int64_t c0 = 8ll * (blockIdx.x % slabs) * blockDim.x;
-  const int64_t c = c0 + 8ll * threadIdx.x;
-  const int64_t lo = block * s.block + static_cast<int64_t>(threadIdx.y) * s.tile;
-  const int64_t hi = min(lo + s.tile, s.n);
   const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const uint32_t block = blockIdx.x / slabs;
+  const uint32_t c0 = 8 * (blockIdx.x % slabs) * blockDim.x;
+  const uint32_t c = c0 + 8 * threadIdx.x;
+  const uint32_t lo = block * s.block + threadIdx.y * s.tile;
+  const uint32_t hi = min(lo + s.tile, s.n);
   Ends mine{kNoKey, kNoKey, 0};
   // (lanes behind the last column stay for the exchange of columns)
   float* warp = nullptr;
-  if (!VEC && blockDim.x >= 32) warp = reinterpret_cast<float*>(smem + kPartBytes) + 8 * (tid & ~31);
+  if (!VEC && blockDim.x >= 32) warp = reinterpret_cast<float*>(smem + Smem::exchange) + 8 * (tid & ~31);
   if (lo < hi && (c < s.dim || warp)) {
-    constexpr int N = kGroup<TD>;
+    constexpr int N = Ring<TD, VEC>::rows;
     DropKey k{};
     if (DROP) k = drop_key(s.drop);
     const Rows<TD, TG, VEC> rows{s, keys, ids, static_cast<const TD*>(s.dy) + c, c, hi,
-                                 static_cast<uint32_t>(__cvta_generic_to_shared(smem + kPartBytes)) + 16 * tid};
+                                 static_cast<uint32_t>(__cvta_generic_to_shared(smem + Smem::ring)) + 16 * tid};
     const uint32_t before = lo > 0 ? keys[lo - 1] : kNoKey;
     const uint32_t behind = hi < s.n ? keys[hi] : kNoKey;
     float acc[8];
@@ -768,26 +810,22 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
 #pragma unroll
     for (int g = 0; g < kStages; ++g) rows.request(lo + g * N, g);
     int stage = 0;
-    for (int64_t i = lo; i < hi; i += N) {
+    for (uint32_t i = lo; i < hi; i += N) {
       rows.arrived();
       uint32_t key[N], pos[N];
       load_ids<N>(keys, i, key);
       if (DROP || !VEC) load_ids<N>(ids, i, pos);
-      Raw8<TD> raw[N];
-#pragma unroll
-      for (int u = 0; u < N; ++u)
-        if (!VEC && i + u < hi && key[u] < s.vocab && c < s.dim) raw[u] = rows.get(stage, u, pos[u]);
 #pragma unroll
       for (int u = 0; u < N; u += 2) {
         Fates<VEC> fates;
-        if (DROP) fates.set({pos[u] * s.dim + c, pos[u + 1] * s.dim + c}, s.drop, k);
+        if (DROP)
+          fates.set({static_cast<uint64_t>(pos[u]) * s.dim + c, static_cast<uint64_t>(pos[u + 1]) * s.dim + c}, s.drop, k);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t id = key[u + h];
           if (i + u + h >= hi || id >= s.vocab) continue;
-          if (VEC) raw[u + h] = rows.get(stage, u + h, pos[u + h]);
-          float v[8];
-          unpack8<TD>(raw[u + h], v);
+          float v[8] = {};
+          if (VEC || c < s.dim) unpack8<TD>(rows.get(stage, u + h, pos[u + h]), v);
           if (id != run) {
             if (run != kNoKey) {
               if (first && run == before) {
@@ -846,7 +884,7 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
         }
         if (!e.through) {
           if (from_before)
-            s.partial[2 * block * s.partial_pitch + c0 + col] = acc;
+            row_at(s.partial, 2 * block, s.partial_pitch)[c0 + col] = acc;
           else
             put_one<TG>(s, e.head, c0 + col, acc);
           open = from_before = false;
@@ -857,7 +895,7 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas)
         open = true;
       }
     }
-    if (open) s.partial[(2 * block + (from_before ? 0 : 1)) * s.partial_pitch + c0 + col] = acc;
+    if (open) row_at(s.partial, 2 * block + (from_before ? 0 : 1), s.partial_pitch)[c0 + col] = acc;
   }
 }
 
@@ -880,27 +918,35 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(SumArgs s) {
   __shared__ float4 sums[kJoinParts][kJoinLanes];
   let_next_start();
   wait_for_previous();
-  const int64_t block = blockIdx.x;
-  const int64_t lo = block * s.block, hi = lo + s.block;
+  const uint32_t block = blockIdx.x;
+  const uint32_t lo = block * s.block, hi = lo + s.block;
   if (hi >= s.n) return;
   const uint32_t key = s.keys[hi - 1], behind = s.keys[hi];
   const uint32_t before = lo > 0 ? s.keys[lo - 1] : kNoKey;
   if (key >= s.vocab || behind != key || before == key) return;
   // the blocks behind this one whose first item has the key are consecutive
   const int tid = threadIdx.y * kJoinLanes + threadIdx.x;
-  int64_t more = 0;
+  int more = 0;
   for (int found = kJoinThreads; found == kJoinThreads; more += found) {
-    const int64_t i = (block + 1 + more + tid) * s.block;
+    const uint64_t i = static_cast<uint64_t>(block + 1 + more + tid) * s.block;
     found = __syncthreads_count(i < s.n && s.keys[i] == key);
   }
-  const int64_t c = 4 * (static_cast<int64_t>(blockIdx.y) * kJoinLanes + threadIdx.x);
+  const uint32_t c = 4 * (blockIdx.y * kJoinLanes + threadIdx.x);
   const bool on = c < s.dim;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (on) {
-#pragma unroll 4
-    for (int64_t j = threadIdx.y; j <= more; j += kJoinParts) {
-      const int64_t row = j == 0 ? 2 * block + 1 : 2 * (block + j);
-      add4(acc, *reinterpret_cast<const float4*>(s.partial + row * s.partial_pitch + c));
+    constexpr int kAhead = 8;  // loads under way
+    for (int j0 = threadIdx.y; j0 <= more; j0 += kAhead * kJoinParts) {
+      float4 v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = j0 + u * kJoinParts;
+        const uint32_t row = j == 0 ? 2 * block + 1 : 2 * (block + j);
+        if (j <= more) v[u] = *reinterpret_cast<const float4*>(row_at(s.partial, row, s.partial_pitch) + c);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (j0 + u * kJoinParts <= more) add4(acc, v[u]);
     }
   }
   sums[threadIdx.y][threadIdx.x] = acc;
@@ -909,9 +955,16 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(SumArgs s) {
 #pragma unroll
   for (int q = 1; q < kJoinParts; ++q) add4(acc, sums[q][threadIdx.x]);
   const float f[4] = {acc.x, acc.y, acc.z, acc.w};
+  TG* at = row_at(static_cast<TG*>(s.grad), key, s.grad_pitch) + c;
+  const int left = static_cast<int>(s.dim - c);
+  float g[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (c + j < s.dim) put_one<TG>(s, key, c + j, f[j]);
+  for (int j = 0; j < 4; ++j) g[j] = s.accumulate && j < left ? to_f32(at[j]) : 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float v = __fmul_rn(f[j], s.scale);
+    if (j < left) at[j] = from_f32<TG>(s.accumulate ? __fadd_rn(g[j], v) : v);
+  }
 }
 
 // ---- host -------------------------------------------------------------------------
@@ -1110,13 +1163,13 @@ bool sizes_ok(int64_t n, int64_t vocab, int64_t dim) {
 template <typename TD, typename TG, bool DROP, bool VEC, bool SMALL>
 int launch_sums(const SumArgs& s, const Fill& f, cudaStream_t st) {
   const Shape sh = shape(s.dim);
-  const int64_t blocks = (s.n + s.block - 1) / s.block;
+  const int64_t blocks = (int64_t{s.n} + s.block - 1) / s.block;
   const int64_t sum_ctas = blocks * sh.slabs;
   const int64_t cta_rows = int64_t{f.per_warp} * kSumThreads / 32;
   const int64_t fill_ctas = f.rows > 0 ? (f.rows + cta_rows - 1) / cta_rows : 0;
   if (sum_ctas + fill_ctas == 0) return DFC_OK;
   const auto kernel = sum_kernel<TD, TG, DROP, VEC, SMALL>;
-  const int smem = kSumSmem + (SMALL ? 8 * kSmallTokens : 0);
+  constexpr int smem = SumSmem<TD, VEC, SMALL>::bytes;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return failed(e);
   e = launch_next(kernel, dim3(static_cast<unsigned>(sum_ctas + fill_ctas)), dim3(sh.lanes, sh.tiles), smem, st,
@@ -1142,8 +1195,8 @@ int run_sums(const SumArgs& s, const Fill& f, cudaStream_t st) {
 template <typename TD, typename TG>
 int by_path(const SumArgs& s, const Fill& f, bool drop, cudaStream_t st) {
   const bool vec = s.dim % 8 == 0 && aligned(s.dy, 16) && aligned(s.grad, 16) &&
-                   s.dy_pitch * static_cast<int64_t>(sizeof(TD)) % 16 == 0 &&
-                   s.grad_pitch * static_cast<int64_t>(sizeof(TG)) % 16 == 0;
+                   s.dy_pitch % (16 / sizeof(TD)) == 0 &&
+                   s.grad_pitch % (16 / sizeof(TG)) == 0;
   if (vec) return drop ? run_sums<TD, TG, true, true>(s, f, st) : run_sums<TD, TG, false, true>(s, f, st);
   return drop ? run_sums<TD, TG, true, false>(s, f, st) : run_sums<TD, TG, false, false>(s, f, st);
 }
@@ -1171,7 +1224,9 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
                                   const DfcDropout* dropout, int32_t* error_flag, void* scratch,
                                   size_t scratch_bytes, void* stream) {
   using namespace dfc;
-  if (!sizes_ok(n_tokens, vocab, dim) || dy_pitch < 0 || grad_pitch < dim) return DFC_ERR_SIZE;
+  if (!sizes_ok(n_tokens, vocab, dim) || dy_pitch < 0 || dy_pitch > DFC_MAX_PITCH || grad_pitch < dim ||
+      grad_pitch > DFC_MAX_PITCH)
+    return DFC_ERR_SIZE;
   if ((token_bytes != 4 && token_bytes != 8) || !known_dtype(dy_dtype) || !known_dtype(grad_dtype))
     return DFC_ERR_DTYPE;
   SumArgs s{};
@@ -1204,15 +1259,15 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
     const int rc = sort_tokens(s.tokens, n_tokens, l, base, &s.keys, &s.pos, st);
     if (rc != DFC_OK) return rc;
   }
-  s.n = n_tokens;
+  s.n = static_cast<uint32_t>(n_tokens);
   s.tile = l.tile;
-  s.block = l.block;
+  s.block = static_cast<uint32_t>(l.block);
   s.dy = dy;
-  s.dy_pitch = dy_pitch;
+  s.dy_pitch = static_cast<uint32_t>(dy_pitch);
   s.grad = grad;
-  s.grad_pitch = grad_pitch;
-  s.vocab = vocab;
-  s.dim = dim;
+  s.grad_pitch = static_cast<uint32_t>(grad_pitch);
+  s.vocab = static_cast<uint32_t>(vocab);
+  s.dim = static_cast<uint32_t>(dim);
   // dropout's scale belongs to every term of the sum: applied once, to the sum
   s.scale = drop ? static_cast<float>(static_cast<double>(scale) * (dropout->p < 1.0 ? 1.0 / (1.0 - dropout->p) : 0.0))
                  : scale;
@@ -1220,7 +1275,7 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   s.wide_dy = aligned(dy, 32) && dy_pitch % 8 == 0;
   s.wide_grad = aligned(grad, 32) && grad_pitch % 8 == 0;
   s.partial = reinterpret_cast<float*>(base + l.partial);
-  s.partial_pitch = l.partial_pitch;
+  s.partial_pitch = static_cast<uint32_t>(l.partial_pitch);
   if (dy_dtype == DFC_DTYPE_F32) return by_grad<float>(s, f, grad_dtype, drop, st);
   if (dy_dtype == DFC_DTYPE_BF16) return by_grad<bf16>(s, f, grad_dtype, drop, st);
   return by_grad<f16>(s, f, grad_dtype, drop, st);

@@ -269,41 +269,65 @@ __device__ __forceinline__ void store8(T* p, const Raw8<T>& r, int wide) {
   q[0] = r.q[0];
 }
 
-// Eight elements from any address, p aligned to T, of an array that occupies
-// [lo, hi): the 16-byte blocks around them and a shift, where the blocks lie
-// within the array, otherwise element by element.  `count` of them are needed;
-// what the others hold is undefined.
+// Eight elements from any address p (aligned to T) of an array that occupies
+// [lo, hi): the 16-byte blocks around them, to be shifted into place.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8_any(const T* p, int count, const void* lo, const void* hi) {
-  constexpr int kBlocks = sizeof(T) / 2 + 1;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p), first = at & ~uintptr_t{15};
-  const uint32_t off = static_cast<uint32_t>(at & 15);
-  Raw8<T> r;
-  if (first >= reinterpret_cast<uintptr_t>(lo) && first + 16 * kBlocks <= reinterpret_cast<uintptr_t>(hi)) {
-    uint32_t w[4 * kBlocks];
+struct Blocks {
+  static constexpr int N = sizeof(T) / 2 + 1;
+  uint4 q[N];
+
+  // The blocks lie within the array.
+  __device__ __forceinline__ static bool within(const T* p, const void* lo, const void* hi) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p) & ~uintptr_t{15};
+    return first >= reinterpret_cast<uintptr_t>(lo) && first + 16 * N <= reinterpret_cast<uintptr_t>(hi);
+  }
+
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4* first = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t{15});
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      const uint4 q = reinterpret_cast<const uint4*>(first)[b];
-      w[4 * b] = q.x, w[4 * b + 1] = q.y, w[4 * b + 2] = q.z, w[4 * b + 3] = q.w;
-    }
-    // down by off bytes: two words, one word, half a word
+    for (int b = 0; b < N; ++b) q[b] = first[b];
+  }
+
+  // The elements: down by p's offset in its block, in steps of two words, one
+  // word and half a word.
+  __device__ __forceinline__ Raw8<T> at(const T* p) const {
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
+    uint32_t w[4 * N];
 #pragma unroll
-    for (int i = 0; i < 4 * kBlocks - 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+    for (int b = 0; b < N; ++b) w[4 * b] = q[b].x, w[4 * b + 1] = q[b].y, w[4 * b + 2] = q[b].z, w[4 * b + 3] = q[b].w;
 #pragma unroll
-    for (int i = 0; i < 4 * kBlocks - 3; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    for (int i = 0; i < 4 * N - 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4 * N - 3; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], off & 2 ? 16 : 0);
     }
+    Raw8<T> r;
 #pragma unroll
-    for (int b = 0; b < kBlocks - 1; ++b) r.q[b] = make_uint4(w[4 * b], w[4 * b + 1], w[4 * b + 2], w[4 * b + 3]);
+    for (int b = 0; b < N - 1; ++b) r.q[b] = make_uint4(w[4 * b], w[4 * b + 1], w[4 * b + 2], w[4 * b + 3]);
     return r;
   }
+};
+
+// The first `count` of eight elements, one by one; the others are zero.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8_single(const T* p, int count) {
   T v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = j < count ? p[j] : T(0.0f);
+  Raw8<T> r;
   memcpy(&r, v, sizeof(r));
   return r;
+}
+
+// Eight elements from any address of [lo, hi).
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8_any(const T* p, const void* lo, const void* hi) {
+  if (!Blocks<T>::within(p, lo, hi)) return load8_single(p, 8);
+  Blocks<T> b;
+  b.load(p);
+  return b.at(p);
 }
 
 inline bool known_dtype(int32_t d) {

@@ -268,7 +268,8 @@ def check_grad(tok, dy, vocab, *, grad_dtype=F32, accumulate=False, padding_idx=
 
 
 SHAPES = [(1, 5, 8), (2, 1, 3), (31, 7, 16), (32, 3, 129), (33, 40, 1000), (300, 511, 64), (4097, 513, 24),
-          (5000, 1000, 72), (700, 70001, 8), (2049, 263000, 16), (20000, 37, 40)]
+          (5000, 1000, 72), (700, 70001, 8), (2049, 263000, 16), (20000, 37, 40),
+          (500, 60, 1001), (1500, 99, 523), (1024, 300, 264), (1025, 300, 264), (257, 9, 2056)]
 
 
 @pytest.mark.parametrize("kind", ["equal", "distinct", "uniform", "skewed", "padded"])
@@ -277,6 +278,36 @@ SHAPES = [(1, 5, 8), (2, 1, 3), (31, 7, 16), (32, 3, 129), (33, 40, 1000), (300,
 def test_embedding_grad(cuda, kind, n, vocab, dim, accumulate):
     tok = draw_tokens(kind, n, vocab, n)
     check_grad(tok, randn((n, dim), F32, dim), vocab, accumulate=accumulate, scale=1.7)
+
+
+@pytest.mark.parametrize("n", [5, 900, 5000])
+@pytest.mark.parametrize("vocab", [(1 << 22) - 1, 1 << 22, 5_000_001])
+def test_embedding_grad_of_large_tables(cuda, n, vocab):
+    """Around the table size up to which every CTA sorts few tokens itself."""
+    tok = draw_tokens("uniform", n, vocab, n)
+    tok[: n // 3] = vocab - 1
+    dy = randn((n, 8), F32, 1)
+    grad = torch.full((vocab, 8), 3.0, device=cuda)
+    t = torch.from_numpy(tok).cuda()
+    kernels.embedding_grad(t, dy, grad)
+    rows = np.unique(tok)
+    want, mag, terms = T.embedding_grad(np.searchsorted(rows, tok), f64(dy), len(rows))
+    assert_close(grad[torch.from_numpy(rows).cuda()], want, F32, HALF32 * (terms[:, None] + 4) * mag)
+    grad[t] = 0
+    assert not grad.any()
+
+
+@pytest.mark.parametrize("shift", [1, 3, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_embedding_grad_alignment(cuda, shift, dtype):
+    """dy and grad that begin anywhere; what lies around grad stays as it was."""
+    n, vocab, dim = 333, 77, 136
+    tok = draw_tokens("skewed", n, vocab, 2)
+    dy = randn(n * dim + 16, dtype, 3)[shift:shift + n * dim].view(n, dim)
+    for accumulate in (False, True):
+        flat = torch.full((vocab * dim + 32,), 7.0, dtype=dtype, device=cuda)
+        check_grad(tok, dy, vocab, grad=flat[shift:shift + vocab * dim].view(vocab, dim), accumulate=accumulate)
+        assert (flat[:shift] == 7).all() and (flat[shift + vocab * dim:] == 7).all()
 
 
 @pytest.mark.parametrize("dy_dtype", [F32, BF16, F16])
@@ -320,6 +351,23 @@ def test_embedding_grad_views(cuda, dim, lead, width):
     check_grad(tok, dy[:1].expand(n, dim), vocab)
     with pytest.raises(ValueError):
         kernels.embedding_grad(torch.from_numpy(tok).cuda(), dy, torch.empty(1, dim, device=cuda).expand(vocab, dim))
+
+
+def test_gradients_of_masked_places_do_not_count(cuda):
+    """NaN and Inf at padding, out-of-range and dropped places stay there."""
+    n, vocab, dim = 300, 20, 64
+    tok = draw_tokens("uniform", n, vocab, 1)
+    tok[::7] = 5                    # the padding row
+    tok[3::11] = vocab + 2          # outside
+    dy = randn((n, dim), F32, 2)
+    keep = torch.from_numpy(T.keep((n, dim), 0.4, 17, 5)).cuda()
+    dy[~keep] = float("nan")
+    dy[torch.from_numpy((tok == 5) | (tok >= vocab)).cuda()] = float("inf")
+    grad = kernels.embedding_grad(torch.from_numpy(tok).cuda(), dy, torch.empty(vocab, dim, device=cuda),
+                                  padding_idx=5, p=0.4, seed=17, offset=5)
+    assert torch.isfinite(grad).all() and (grad[5] == 0).all()
+    with pytest.raises(IndexError):
+        kernels.check_tokens(cuda)
 
 
 def test_embedding_grad_edges(cuda):
@@ -470,6 +518,35 @@ def test_second_derivatives_of_the_lookup(cuda):
     w.grad = torch.zeros_like(w)
     with pytest.raises(RuntimeError):
         nn.embedding(tok, w, 2.0, grad_in_place=True).sum().backward(create_graph=True)
+
+
+def test_in_place_gradient_in_the_sharded_optimizer(cuda):
+    """ShardedDFCAdamW owns .grad (a view of its flat buffer): the table's rows
+    are added there, and the step is the one that a dense gradient gives."""
+    import torch.distributed as dist
+
+    from t3st_b200.zero import ShardedDFCAdamW
+
+    made = not dist.is_initialized()
+    if made:
+        dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        tok = torch.randint(0, 120, (3, 40), generator=torch.Generator().manual_seed(1)).cuda()
+        finals = []
+        for in_place in (False, True):
+            torch.manual_seed(0)
+            net = nn.Embedding(120, 48, padding_idx=0, scale=2.0, grad_in_place=in_place).cuda()
+            opt = ShardedDFCAdamW(net.parameters(), lr=1e-2, weight_decay=0.01)
+            for _ in range(3):
+                opt.zero_grad()
+                net(tok).square().mean().backward()
+                assert net.weight.grad.data_ptr() == opt.flat_grad.data_ptr()
+                opt.step()
+            finals.append(net.weight.detach().clone())
+        assert torch.equal(*finals)
+    finally:
+        if made:
+            dist.destroy_process_group()
 
 
 def test_in_place_gradient_accumulates(cuda):

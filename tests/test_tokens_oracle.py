@@ -76,7 +76,7 @@ def test_embedding_refusals():
                                  flag, None)
 
     for bad in (dict(n=-1), dict(n=(1 << 28) + 1), dict(vocab=-1), dict(vocab=(1 << 30) + 1),
-                dict(dim=-1), dict(dim=(1 << 20) + 1), dict(pitch=-1), dict(n=1 << 28, dim=1 << 12)):
+                dict(dim=-1), dict(dim=(1 << 20) + 1), dict(pitch=-1), dict(pitch=1 << 31), dict(n=1 << 28, dim=1 << 12)):
         assert f(**bad) == _lib.DFC_ERR_SIZE, bad
     for bad in (dict(tb=2), dict(tdt=4), dict(odt=-1)):
         assert f(**bad) == _lib.DFC_ERR_DTYPE, bad
@@ -103,7 +103,7 @@ def test_embedding_grad_refusals():
                                       1.0, -1, 0, drop, flag, scratch, nbytes, None)
 
     for bad in (dict(n=-1), dict(n=(1 << 28) + 1), dict(vocab=-1), dict(dim=-1), dict(dpitch=-1),
-                dict(gpitch=15), dict(n=1 << 28, dim=1 << 12, gpitch=1 << 12)):
+                dict(dpitch=1 << 31), dict(gpitch=1 << 31), dict(gpitch=15), dict(n=1 << 28, dim=1 << 12, gpitch=1 << 12)):
         assert f(**bad) == _lib.DFC_ERR_SIZE, bad
     for bad in (dict(tb=1), dict(ddt=3), dict(gdt=9)):
         assert f(**bad) == _lib.DFC_ERR_DTYPE, bad
