@@ -325,6 +325,10 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         all += c;
       }
     }
+    const bool last = p + 1 == passes;
+    // nothing of this CTA's shared memory is read by others after this: they
+    // meet again before the first one leaves
+    if (last) cluster.barrier_arrive();
     const uint32_t own_inc = warp_inclusive(own), all_inc = warp_inclusive(all);
     if (lane == 31) {
       warp_own[warp] = own_inc;
@@ -348,7 +352,6 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
       }
     }
     __syncthreads();
-    const bool last = p + 1 == passes;
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
       const uint32_t i = threadIdx.x + r * kClusterThreads;
@@ -363,8 +366,10 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         }
       }
     }
-    cluster.sync();  // the items have arrived; no CTA leaves while others read its counts
-    if (!last) {
+    if (last) {
+      cluster.barrier_wait();
+    } else {
+      cluster.sync();  // the items have arrived
 #pragma unroll
       for (int r = 0; r < ITEMS; ++r) {
         if (item0 + 32 * r < here) {

@@ -590,6 +590,42 @@ def test_captured_steps_replay_like_eager_ones(cuda):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_captured_backward_into_existing_gradients(cuda, in_place):
+    rng, net = make(in_place)
+    tok = torch.randint(0, 120, (4, 32), device=cuda)
+    dy = randn((4, 32, 48), BF16, 7)
+    for p in net.parameters():
+        p.grad = torch.zeros_like(p)
+
+    def step():
+        for p in net.parameters():
+            p.grad.zero_()
+        net(tok).backward(dy)
+        rng.advance()
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    eager = []
+    rng.state[1] = 0
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            step()
+            eager.append([p.grad.clone() for p in net.parameters()])
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        step()
+    rng.state[1] = 0
+    for want in eager:
+        graph.replay()
+        assert all(torch.equal(p.grad, g) for p, g in zip(net.parameters(), want))
+
+
 def test_other_streams(cuda):
     tok = torch.randint(0, 1000, (5000,), device=cuda)
     dy = randn((5000, 256), BF16, 1)
