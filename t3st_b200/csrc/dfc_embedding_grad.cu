@@ -662,40 +662,31 @@ template <typename TD, bool VEC, bool SMALL>
 struct SumSmem {
   static constexpr int exchange = kPartBytes + kEndsBytes;
   static constexpr int tokens = exchange + (VEC ? 0 : kExchangeBytes);
-  static constexpr int ring = tokens + (SMALL ? 8 * 4 * kSumThreads : 0);
+  static constexpr int ring = tokens + (SMALL ? 8 * 2 * kSumThreads : 0);
   static constexpr int bytes = ring + Ring<TD, VEC>::bytes;
 };
 constexpr int kSumCtas = 3;  // per SM
 
 // ---- up to kSmallTokens tokens: one CTA sorts them alone -----------------------
-constexpr int kSmallTokens = 4 * kSumThreads;
-constexpr int kSmallBits = 10;  // of a position
+constexpr int kSmallTokens = 2 * kSumThreads;
+constexpr int kSmallBits = 9;  // of a position
 constexpr int64_t kSmallVocab = int64_t{1} << (32 - kSmallBits);
 
-__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b, bool up) {
-  const uint32_t lo = min(a, b), hi = max(a, b);
-  a = up ? lo : hi;
-  b = up ? hi : lo;
-}
-
-// Bitonic sort of kSumThreads * E words key << 10 | position, E consecutive
-// ones a thread: distances within a thread in registers, within a warp by
+// Bitonic sort of kSumThreads * E words key << kSmallBits | position, E (one or
+// two) consecutive ones a thread: distances within a thread in registers, within a warp by
 // shuffles, the others through `words` in shared memory.  All words differ
 // (padding aside), so the order is by key, then position.
 template <int E>
-__device__ __noinline__ void small_sort(uint32_t (&x)[4], uint32_t* words, int tid) {
+__device__ __noinline__ void small_sort(uint32_t (&x)[2], uint32_t* words, int tid) {
 #pragma unroll 1
   for (int k = 2; k <= kSumThreads * E; k <<= 1) {
 #pragma unroll 1
     for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j < E) {
-        if (E >= 2 && j == 1) {
-          exchange(x[0], x[1], (tid * E & k) == 0);
-          if (E == 4) exchange(x[2], x[3], (tid * E + 2 & k) == 0);
-        } else if (E == 4) {
-          exchange(x[0], x[2], (tid * E & k) == 0);
-          exchange(x[1], x[3], (tid * E & k) == 0);
-        }
+      if (j < E) {  // E = 2
+        const uint32_t lo = min(x[0], x[1]), hi = max(x[0], x[1]);
+        const bool up = (tid * E & k) == 0;
+        x[0] = up ? lo : hi;
+        x[1] = up ? hi : lo;
         continue;
       }
       if (j >= 32 * E) {
@@ -718,22 +709,20 @@ __device__ __noinline__ void small_sort(uint32_t (&x)[4], uint32_t* words, int t
 // of four: read, not used, behind n).
 __device__ __forceinline__ void small_sort_tokens(const Tokens& tk, int n, uint32_t* keys, uint32_t* pos) {
   const int tid = threadIdx.y * blockDim.x + threadIdx.x;
-  const int e = n <= kSumThreads ? 1 : n <= 2 * kSumThreads ? 2 : 4;  // items a thread
-  uint32_t x[4];
+  const int e = n <= kSumThreads ? 1 : 2;  // items a thread
+  uint32_t x[2];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
     const int t = tid * e + j;
     x[j] = j < e && t < n ? token_key(tk, t) << kSmallBits | t : 0xFFFFFFFFu;
   }
   if (e == 1)
     small_sort<1>(x, keys, tid);
-  else if (e == 2)
-    small_sort<2>(x, keys, tid);
   else
-    small_sort<4>(x, keys, tid);
+    small_sort<2>(x, keys, tid);
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
     if (j < e) {
       keys[tid * e + j] = x[j] >> kSmallBits;
       pos[tid * e + j] = x[j] & ((1u << kSmallBits) - 1);
@@ -1187,8 +1176,10 @@ int launch_sums(const SumArgs& s, const Fill& f, cudaStream_t st) {
   return e == cudaSuccess ? launch_status() : failed(e);
 }
 
-// Every CTA sorts the tokens itself: one launch less, 17.2 -> 14.2 us for 300
-// tokens of 384 FP32 columns.
+// Every CTA sorts the tokens itself, one launch less: 16.7 -> 13.8 us for 300
+// tokens of 384 FP32 columns, 18.7 -> 14.8 for 400 of 4,096 bf16 ones.  Up to
+// 1,024 tokens it cost more where rows are wide (24.6 instead of 20.7 us for 600
+// of 4,096) and gained at most 2 us elsewhere.
 bool small(int64_t n, int64_t vocab) { return n <= kSmallTokens && vocab < kSmallVocab; }
 
 template <typename TD, typename TG, bool DROP, bool VEC>
