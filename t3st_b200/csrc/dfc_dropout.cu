@@ -7,19 +7,25 @@
 // 16-byte access per 16-bit operand and group.  One CTA per tile of consecutive
 // groups, in address order (the shape dfc_compress_ef measured best), all
 // loads issued before the first is used.
+//
+// Bounds (B200, 2^26 elements): FP32 with residual runs at the HBM floor of the
+// measured copy bandwidth (123 us), bf16 with residual too (60 us under ncu,
+// floor 61.5; 19 to 22 instructions an element).  bf16 without residual takes
+// about 52 us where HBM would need 41: there the ten rounds bound it, their
+// multiplications most of all.
 #include "dfc_philox.cuh"
 
 namespace dfc {
 namespace {
 
 constexpr int kThreads = 256;
-#ifndef DFC_DROP_GROUPS
-#define DFC_DROP_GROUPS 2
-#endif
-#ifndef DFC_DROP_BLOCKS
-#define DFC_DROP_BLOCKS 4
-#endif
-constexpr int kGroups = DFC_DROP_GROUPS;  // groups per thread
+// Groups per thread: two for 16-bit types, one for FP32 (32 bytes of each
+// operand in flight per thread either way), and registers for 6 CTAs per SM.
+// Of 1, 2 and 4 groups at 3 to 6 CTAs, 2^26 elements with residual, launch
+// included: bf16 65.5 us (1 group 73.7; 4 groups 65.5 at 3 CTAs, but 8.2 us
+// instead of 6.2 for 2^16 elements), FP32 122.9 us (2 groups 124.9, 4 groups 132).
+template <typename T>
+constexpr int kGroups = sizeof(T) == 2 ? 2 : 1;
 
 // Element accesses of group g, for any alignment and for a last group of
 // fewer than eight elements.
@@ -42,13 +48,14 @@ __device__ __forceinline__ void drop_group(const T* x, const T* res, T* y, int64
 
 // x, res and y on 16-byte boundaries.
 template <typename T, bool RES, bool DROP>
-__global__ void __launch_bounds__(kThreads, DFC_DROP_BLOCKS)
+__global__ void __launch_bounds__(kThreads, 6)
     dropout_vec_kernel(const T* x, const T* res, T* y, int64_t n, int wide, DropArgs a) {
+  constexpr int G = kGroups<T>;
   const int64_t groups = n / 8;
-  const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kGroups) + threadIdx.x;
-  Raw8<T> X[kGroups], R[kGroups];
+  const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (kThreads * G) + threadIdx.x;
+  Raw8<T> X[G], R[G];
 #pragma unroll
-  for (int u = 0; u < kGroups; ++u) {
+  for (int u = 0; u < G; ++u) {
     const int64_t g = g0 + u * kThreads;
     if (g < groups) {
       X[u] = load8(x + 8 * g, wide);
@@ -56,16 +63,16 @@ __global__ void __launch_bounds__(kThreads, DFC_DROP_BLOCKS)
     }
   }
   DropKey k{};
-  uint4 w[kGroups];
+  uint4 w[G];
   if (DROP) {
     k = drop_key(a);
-    uint64_t g[kGroups];
+    uint64_t g[G];
 #pragma unroll
-    for (int u = 0; u < kGroups; ++u) g[u] = g0 + u * kThreads;
-    drop_words<kGroups>(g, a, k, w);
+    for (int u = 0; u < G; ++u) g[u] = g0 + u * kThreads;
+    drop_words<G>(g, a, k, w);
   }
 #pragma unroll
-  for (int u = 0; u < kGroups; ++u) {
+  for (int u = 0; u < G; ++u) {
     const int64_t g = g0 + u * kThreads;
     if (g < groups) {
       float v[8];
@@ -99,7 +106,7 @@ int launch(const void* x, const void* res, void* y, int64_t n, const DropArgs& a
   T* py = static_cast<T*>(y);
   const int64_t groups = (n + 7) / 8;
   const bool vec = aligned(x, 16) && aligned(res, 16) && aligned(y, 16);
-  const int64_t tile = vec ? kThreads * kGroups : kThreads;
+  const int64_t tile = vec ? kThreads * kGroups<T> : kThreads;
   const unsigned grid = static_cast<unsigned>((groups + tile - 1) / tile);
   if (vec)
     dropout_vec_kernel<T, RES, DROP><<<grid, kThreads, 0, st>>>(

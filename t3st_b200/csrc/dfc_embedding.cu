@@ -8,13 +8,20 @@
 // 16-byte pieces the table is read in such pieces; otherwise from the 16-byte
 // blocks around the elements, shifted into place, and element by element where
 // a group spans rows.
+//
+// Bounds (B200, 16,384 tokens of 4,096 columns, FP32 table of 131,072 rows to
+// bf16): without dropout 53 us, 0.92 of the copy bandwidth counting each named
+// row once; with it 68 us, held by instructions (27 per element, 3.0 a cycle and
+// SM), not by HBM.
 #include "dfc_philox.cuh"
 
 namespace dfc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = 2;  // groups per thread; with registers for 6 CTAs per SM
+// Groups per thread, with registers for 6 CTAs per SM.  The case above with
+// dropout: 73.7 us (launch included; 1 group 88.0, 4 groups 77.8 at 4 CTAs).
+constexpr int kGroups = 2;
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_t t) {
   return wide ? static_cast<const int64_t*>(tokens)[t]

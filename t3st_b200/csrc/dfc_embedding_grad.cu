@@ -15,6 +15,13 @@
 // Up to kSmallTokens, step 1 is left out: every CTA of the sums sorts the
 // tokens for itself.
 // No atomics on floats: the same inputs give the same bits.
+//
+// Bounds (B200).  65,539 bf16 rows of 4,096 into an FP32 table of 131,072 rows:
+// 412 us for 2.63 GB, 0.98 of the copy bandwidth (sort 31, sums and zeros 367,
+// joins 7).  32,768 rows of 2,048, dropout on, added to a table of 32,768 rows:
+// 97 us (sort 14, sums 76, joins 8), the sums held by the masks' instructions
+// (25 per element); without dropout 76 us.  Small calls are chains of launches
+// and latencies: 14 us for 300 tokens.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -665,7 +672,7 @@ struct SumSmem {
   static constexpr int ring = tokens + (SMALL ? 8 * 2 * kSumThreads : 0);
   static constexpr int bytes = ring + Ring<TD, VEC>::bytes;
 };
-constexpr int kSumCtas = 3;  // per SM
+constexpr int kSumCtas = 3;  // per SM; 4 (64 registers) measured the same within 2%
 
 // ---- up to kSmallTokens tokens: one CTA sorts them alone -----------------------
 constexpr int kSmallTokens = 2 * kSumThreads;
@@ -977,6 +984,9 @@ Shape shape(int64_t dim) {
 }
 
 // K: enough threads for every SM, no more ends of tiles than that takes.
+// Measured with 77,000 / 153,600 / 307,000 / 614,000 threads wanted: 32,768 rows
+// of 2,048 with dropout 134 / 119 / 105 / 109 us, 32,768 rows of 1,536 of which
+// half are one token 85 / 73 / 75 / 81 us.
 constexpr int kMinTile = 8, kMaxTile = 256;
 constexpr int64_t kThreadsWanted = 300000;
 
