@@ -81,6 +81,8 @@ __device__ __forceinline__ int64_t row_of(int64_t i, uint64_t per_d) {
   return per_d ? static_cast<int64_t>(__umul64hi(static_cast<uint64_t>(i), per_d)) : i;
 }
 
+// Rows of any width, one group a thread (two a thread, their blocks asked for
+// together: 20.5 instead of 16.4 us for 8,192 FP32 rows of 1,001 to bf16).
 template <typename TT, typename TO, bool DROP>
 __global__ void __launch_bounds__(kThreads)
     embed_any_kernel(const void* tokens, int wide, const TT* table, int64_t pitch, int64_t vocab,

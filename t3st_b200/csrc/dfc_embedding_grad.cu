@@ -1240,7 +1240,7 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   const int rc = make_drop_args(dropout, &s.drop, &drop);
   if (rc != DFC_OK) return rc;
   if (dim == 0) return DFC_OK;
-  if ((!grad && vocab > 0) || !scratch || (n_tokens > 0 && (!tokens || !dy))) return DFC_ERR_NULL;
+  if ((!grad && vocab > 0) || (n_tokens > 0 && (!tokens || !dy || !scratch))) return DFC_ERR_NULL;
   if (!aligned(tokens, token_bytes) || !aligned(dy, dtype_size(dy_dtype)) ||
       !aligned(grad, dtype_size(grad_dtype)) || !aligned(error_flag, 4) || !aligned(scratch, 16))
     return DFC_ERR_ALIGN;

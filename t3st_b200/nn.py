@@ -59,10 +59,12 @@ class CounterRng(torch.nn.Module):
 
 
 def _generator(seed):
-    """(seed, state) of a seed argument: an int, a CounterRng or its tensor."""
-    if isinstance(seed, int):
-        return seed, None
-    return 0, seed.state if isinstance(seed, CounterRng) else seed
+    """(seed, state) of a seed argument: an integer, a CounterRng or its tensor."""
+    if isinstance(seed, CounterRng):
+        return 0, seed.state
+    if isinstance(seed, torch.Tensor):
+        return 0, seed
+    return seed, None
 
 
 def dropout(x: torch.Tensor, p: float, *, seed=0, offset: int = 0,
@@ -101,7 +103,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
 
 class Dropout(torch.nn.Module):
     """Dropout at one site of a :class:`CounterRng`; identity (plus the
-    residual) in eval mode."""
+    residual) in eval mode.  Called twice between two ``advance()``, it draws
+    the same mask twice: give each place of a step a module of its own."""
 
     def __init__(self, p: float, rng: CounterRng):
         super().__init__()

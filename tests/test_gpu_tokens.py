@@ -155,6 +155,7 @@ def test_generator_state_on_the_device(cuda):
             want = nn.dropout(x, 0.3, seed=(1 << 64) - 12345, offset=(step << 32) + site)
             assert torch.equal(m(x), want)
         rng.advance()
+    assert torch.equal(nn.dropout(x, 0.3, seed=np.int64(5)), nn.dropout(x, 0.3, seed=5))
     y = drop(x)
     rng.advance()
     with pytest.raises(RuntimeError):  # the mask of the forward is gone

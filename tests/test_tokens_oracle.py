@@ -114,6 +114,7 @@ def test_embedding_grad_refusals():
                 dict(flag=0x40001), dict(scratch=0x50008)):
         assert f(**bad) == _lib.DFC_ERR_ALIGN, bad
     assert f(nbytes=need - 1) == _lib.DFC_ERR_SCRATCH
+    assert f(n=0, vocab=0, tokens=None, dy=None, grad=None, scratch=None, nbytes=0) == _lib.DFC_OK
     assert f(dim=0) == _lib.DFC_OK
 
 
