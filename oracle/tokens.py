@@ -1,4 +1,4 @@
-"""CPU checker of the token-table and dropout operators, in 64-bit floats.
+"""CPU oracle of the token-table and dropout operators, in 64-bit floats.
 
 Masks: Philox4x32-10 (Salmon et al., SC 2011) on NumPy words, written from
 the published round function; element i of a tensor is kept when its 32-bit

@@ -37,7 +37,7 @@ NVCC_FLAGS = [
     # exactly like the reference's separate eager ops
     "-fmad=false", "-prec-div=true", "-prec-sqrt=true", "-ftz=false",
     "-Xcompiler", "-fPIC,-O2,-fvisibility=hidden",
-    "-shared", "-cudart", "static",
+    "-shared", "-cudart", "static", "--threads", "8",
 ]
 
 

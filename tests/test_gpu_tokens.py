@@ -233,6 +233,27 @@ def test_tokens_outside_the_table(cuda, dim):
     assert np.array_equal(f64(grad), want)  # one term a row
 
 
+def test_errors_reach_the_caller(cuda):
+    """A token outside the table, met by the forward, raises in the backward;
+    a status of the C ABI raises DfcError, in the backward too."""
+    from t3st_b200._lib import DFC_ERR_SIZE, DfcError
+
+    w = randn((10, 8), F32, 1).requires_grad_()
+    out = nn.embedding(torch.tensor([1, 11], device=cuda), w)
+    torch.cuda.synchronize()
+    with pytest.raises(IndexError):
+        out.sum().backward()
+    far = torch.empty((1 << 31) + 64, dtype=BF16, device=cuda).as_strided((2, 8), (1 << 31, 1))
+    with pytest.raises(DfcError) as e:
+        nn.embedding(torch.tensor([0], device=cuda), far)
+    assert e.value.status == DFC_ERR_SIZE
+    far.zero_()
+    out = nn.embedding(torch.tensor([0, 1], device=cuda), w.detach().to(BF16).requires_grad_())
+    with pytest.raises(DfcError):
+        out.backward(far)
+    assert torch.equal(nn.embedding(torch.tensor([3], device=cuda), w), w[3:4])
+
+
 # ---- gradient ----------------------------------------------------------------
 
 def draw_tokens(kind, n, vocab, seed):
