@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import numpy as np
 
@@ -155,23 +156,29 @@ def lib() -> ctypes.CDLL:
 
 
 _host = None
+_host_lock = threading.RLock()
 
 
 def host():
     """The native host module (t3st_b200._dfc_host), built first if it is
-    absent (needs g++ and PyTorch's headers)."""
+    absent (needs g++ and PyTorch's headers).  It is published only once it
+    holds the kernels' addresses: loading the library can fail, and lets other
+    threads run meanwhile."""
     global _host
     if _host is None:
         import importlib
 
         import torch  # noqa: F401  (the extension links against libtorch_python)
 
-        if not os.path.exists(_build.HOST_PATH):
-            _build.build_host()
-        _host = importlib.import_module("t3st_b200._dfc_host")
-        _host.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in
-                     ("dfc_dropout", "dfc_embedding", "dfc_embedding_grad_scratch_bytes",
-                      "dfc_embedding_grad")), check)
+        with _host_lock:
+            if _host is None:
+                if not os.path.exists(_build.HOST_PATH):
+                    _build.build_host()
+                module = importlib.import_module("t3st_b200._dfc_host")
+                module.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in
+                              ("dfc_dropout", "dfc_embedding", "dfc_embedding_grad_scratch_bytes",
+                               "dfc_embedding_grad")), check)
+                _host = module
     return _host
 
 

@@ -41,6 +41,11 @@ decltype(&dfc_embedding_grad_scratch_bytes) f_scratch = nullptr;
 decltype(&dfc_embedding_grad) f_grad = nullptr;
 PyObject* check_status = nullptr;  // _lib.check(name, status): raises
 
+// Before anything else in a call: the addresses are there (set together).
+void check_bound() {
+  TORCH_CHECK(f_grad, "t3st_b200._dfc_host is not bound to the kernels; use it through t3st_b200._lib.host()");
+}
+
 // A non-zero status as the exception of the Python layer.
 void check(const char* name, int status) {
   if (status == DFC_OK) return;
@@ -132,6 +137,7 @@ int32_t* flag_of(const at::Device& dev) {
 
 // ---- the calls -----------------------------------------------------------------
 void run_dropout(const Tensor& x, const Tensor& residual, const Tensor& out, const Mask& m) {
+  check_bound();
   if (residual.defined()) check_devices({&x, &out, &residual});
   else check_devices({&x, &out});
   const int32_t code = dtype_code(x, "x");
@@ -164,6 +170,7 @@ int64_t row_pitch(const Tensor& t, const char* what) {
 }
 
 void run_embedding(const Tensor& tokens, const Tensor& table, const Tensor& out, double scale, const Mask& m) {
+  check_bound();
   check_devices({&tokens, &table, &out});
   const int32_t wide = token_bytes(tokens);
   const int64_t pitch = row_pitch(table, "table"), vocab = table.size(0), dim = table.size(1);
@@ -189,6 +196,7 @@ int64_t padding_row(std::optional<int64_t> padding_idx, int64_t vocab) {
 
 void run_grad(const Tensor& tokens, const Tensor& dy, const Tensor& grad, double scale, int64_t padding,
               const Mask& m, bool accumulate) {
+  check_bound();
   check_devices({&tokens, &dy, &grad});
   const int32_t wide = token_bytes(tokens);
   const int64_t n = tokens.numel();
