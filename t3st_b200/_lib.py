@@ -20,6 +20,8 @@ LIB_PATH = _build.LIB_PATH
 
 # ---- status codes / enums (mirror include/dfc_b200.h) ----
 ABI_VERSION = 4
+# of the native host module's functions (t3st_b200/csrc/dfc_host_plan.cpp)
+HOST_VERSION = 1
 DFC_OK = 0
 DFC_ERR_NULL = -1
 DFC_ERR_ALIGN = -2
@@ -155,13 +157,23 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def _host_is_current() -> bool:
+    """The extension is there and carries this version's mark.  The file is
+    read, not loaded: a process cannot load it again after a rebuild."""
+    try:
+        with open(_build.HOST_PATH, "rb") as f:
+            return b"t3st_b200._dfc_host version %d\0" % HOST_VERSION in f.read()
+    except FileNotFoundError:
+        return False
+
+
 _host = None
 _host_lock = threading.RLock()
 
 
 def host():
     """The native host module (t3st_b200._dfc_host), built first if it is
-    absent (needs g++ and PyTorch's headers).  It is published only once it
+    absent or of another version (needs g++ and PyTorch's headers).  It is published only once it
     holds the kernels' addresses: loading the library can fail, and lets other
     threads run meanwhile."""
     global _host
@@ -172,8 +184,10 @@ def host():
 
         with _host_lock:
             if _host is None:
-                if not os.path.exists(_build.HOST_PATH):
-                    _build.build_host()
+                if not _host_is_current():
+                    _build.build_host(force=True)
+                    if not _host_is_current():
+                        raise ImportError(f"{_build.HOST_PATH}: not version {HOST_VERSION}")
                 module = importlib.import_module("t3st_b200._dfc_host")
                 module.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in
                               ("dfc_dropout", "dfc_embedding", "dfc_embedding_grad_scratch_bytes",

@@ -502,6 +502,9 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_dfc_host",
 
 }  // namespace
 
+// The mark that t3st_b200/_lib.py (HOST_VERSION) looks for in the built file.
+constexpr char kVersion[] = "t3st_b200._dfc_host version 1";
+
 PyMODINIT_FUNC PyInit__dfc_host(void) {
   PlanType.tp_name = "t3st_b200._dfc_host.StepPlan";
   PlanType.tp_basicsize = sizeof(Plan);
@@ -523,6 +526,10 @@ PyMODINIT_FUNC PyInit__dfc_host(void) {
   if (!k_params || !k_param_groups || !k_step || !k_lr || !k_betas || !k_eps || !k_wd) return nullptr;
   PyObject* m = PyModule_Create(&module_def);
   if (!m) return nullptr;
+  if (PyModule_AddStringConstant(m, "version", kVersion) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
   Py_INCREF(&PlanType);
   if (PyModule_AddObject(m, "StepPlan", reinterpret_cast<PyObject*>(&PlanType)) < 0) {
     Py_DECREF(&PlanType);

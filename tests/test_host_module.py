@@ -91,3 +91,57 @@ print("refused")
 """
     out = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip() == "refused", out.stderr
+
+
+def test_a_host_module_of_another_version_is_rebuilt(monkeypatch, tmp_path):
+    """An extension left by an earlier version of the sources is found out
+    before it is imported, and built again."""
+    from t3st_b200 import build
+
+    real, stale = build.HOST_PATH, tmp_path / "old.so"
+    source = tmp_path / "old.c"
+    builds = []
+
+    def rebuild(force=False):
+        builds.append(force)
+        stale.unlink()
+        stale.symlink_to(real)
+        return str(stale)
+
+    for text, want in (("int some_other_symbol;", [True]),
+                       ('const char* v(void) { return "t3st_b200._dfc_host version 0"; }', [True])):
+        source.write_text(text)
+        if stale.is_symlink():
+            stale.unlink()
+        subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(stale), str(source)], check=True)
+        builds.clear()
+        monkeypatch.setattr(build, "HOST_PATH", str(stale))
+        monkeypatch.setattr(build, "build_host", rebuild)
+        monkeypatch.setattr(_lib, "_host", None)
+        assert _lib.host().__name__ == "t3st_b200._dfc_host"
+        assert builds == want
+
+
+def test_a_current_host_module_is_not_rebuilt(monkeypatch):
+    from t3st_b200 import build
+
+    def rebuild(force=False):
+        raise AssertionError("built again")
+
+    monkeypatch.setattr(build, "build_host", rebuild)
+    monkeypatch.setattr(_lib, "_host", None)
+    assert hasattr(_lib.host(), "StepPlan")
+
+
+def test_a_host_module_that_stays_wrong_raises(monkeypatch, tmp_path):
+    from t3st_b200 import build
+
+    source, other = tmp_path / "old.c", tmp_path / "old.so"
+    source.write_text("int some_other_symbol;")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(other), str(source)], check=True)
+    monkeypatch.setattr(build, "HOST_PATH", str(other))
+    monkeypatch.setattr(build, "build_host", lambda force=False: str(other))
+    monkeypatch.setattr(_lib, "_host", None)
+    with pytest.raises(ImportError):
+        _lib.host()
+    assert _lib._host is None
