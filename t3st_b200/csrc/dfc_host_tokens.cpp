@@ -21,6 +21,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
+#include <atomic>
 #include <cstdint>
 #include <cstring>
 #include <mutex>
@@ -103,36 +104,36 @@ void* stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(
 
 // ---- tokens outside the table ------------------------------------------------
 // One int per device in pinned host memory that the kernels set and the next
-// call reads, without waiting.
+// call reads, without waiting.  Backward passes read it from autograd's threads,
+// without the interpreter's lock.
 constexpr int kDevices = 64;
 std::mutex flag_mutex;
-std::array<Tensor, kDevices> flag_memory;
-std::array<volatile int32_t*, kDevices> flags{};
+std::array<Tensor, kDevices> flag_memory;  // under the mutex
+std::array<std::atomic<int32_t*>, kDevices> flags{};
 
+// Of several threads, one reports.
 void check_flag(int device) {
-  volatile int32_t* f = device >= 0 && device < kDevices ? flags[device] : nullptr;
-  if (f && *f) {
-    *f = 0;
-    TORCH_CHECK_INDEX(false, "an earlier call was given a token outside [0, vocab): "
-                             "its rows are NaN, its gradient lacks those tokens");
-  }
+  int32_t* f = device >= 0 && device < kDevices ? flags[device].load(std::memory_order_acquire) : nullptr;
+  TORCH_CHECK_INDEX(!(f && __atomic_load_n(f, __ATOMIC_RELAXED) && __atomic_exchange_n(f, 0, __ATOMIC_RELAXED)),
+                    "an earlier call was given a token outside [0, vocab): "
+                    "its rows are NaN, its gradient lacks those tokens");
 }
 
 int32_t* flag_of(const at::Device& dev) {
   const int i = dev.index();
   TORCH_CHECK(i >= 0 && i < kDevices, "device index out of range");
-  if (!flags[i]) {
+  if (!flags[i].load(std::memory_order_acquire)) {
     std::lock_guard<std::mutex> lock(flag_mutex);
-    if (!flags[i]) {
+    if (!flags[i].load(std::memory_order_relaxed)) {
       TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
                   "call the token-table operators once on this device before capturing them: "
                   "the first call allocates pinned memory");
       flag_memory[i] = at::zeros({1}, at::TensorOptions().dtype(at::kInt)).pin_memory();
-      flags[i] = flag_memory[i].data_ptr<int32_t>();
+      flags[i].store(flag_memory[i].data_ptr<int32_t>(), std::memory_order_release);
     }
   }
   check_flag(i);
-  return const_cast<int32_t*>(flags[i]);
+  return flags[i].load(std::memory_order_acquire);
 }
 
 // ---- the calls -----------------------------------------------------------------
