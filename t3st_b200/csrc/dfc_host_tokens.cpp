@@ -162,7 +162,10 @@ int32_t token_bytes(const Tensor& tokens) {
   return static_cast<int32_t>(tokens.element_size());
 }
 
-bool row_matrix(const Tensor& t) { return t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1); }
+// (Without elements any strides will do; contiguous() would not change them.)
+bool row_matrix(const Tensor& t) {
+  return t.dim() == 2 && (t.numel() == 0 || t.size(1) <= 1 || t.stride(1) == 1);
+}
 
 // Elements between the rows of a matrix whose rows are contiguous.
 int64_t row_pitch(const Tensor& t, const char* what) {

@@ -1,11 +1,14 @@
 """Host side of the token-table and dropout operators on a GPU: threads,
-streams, autograd's bookkeeping."""
+streams, autograd's bookkeeping, empty batches."""
 
 import os
 import subprocess
 import sys
 
 import pytest
+import torch
+
+from t3st_b200 import kernels, nn
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +68,35 @@ print("right")
 """
     out = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip() == "right", out.stderr
+
+
+@pytest.mark.parametrize("tokens,vocab,dim", [((0,), 6, 8), ((0,), 6, 5), ((0,), 0, 8), ((0, 3), 6, 8),
+                                              ((2, 0), 6, 8), ((0,), 6, 0)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_backward_of_an_empty_batch(cuda, tokens, vocab, dim, in_place):
+    """The gradient that sum() sends back is expanded: its strides are zero."""
+    w = torch.randn(vocab, dim, device=cuda).requires_grad_()
+    if in_place:
+        w.grad = torch.ones_like(w)
+    y = nn.embedding(torch.zeros(tokens, dtype=torch.int64, device=cuda), w, 2.0, p=0.1, seed=1,
+                     grad_in_place=in_place)
+    y.sum().backward()
+    assert y.shape == (*tokens, dim) and w.grad.shape == w.shape
+    assert torch.equal(w.grad, torch.ones_like(w) if in_place else torch.zeros_like(w))
+
+
+def test_second_derivative_of_an_empty_batch(cuda):
+    w = torch.randn(6, 8, device=cuda).requires_grad_()
+    dy = torch.zeros(0, 8, device=cuda).requires_grad_()
+    y = nn.embedding(torch.zeros(0, dtype=torch.int64, device=cuda), w)
+    (dw,) = torch.autograd.grad(y, w, dy, create_graph=True)
+    dw.sum().backward()
+    assert dy.grad.shape == (0, 8) and torch.equal(dw, torch.zeros_like(w))
+
+
+def test_rows_of_empty_matrices_lie_anywhere(cuda):
+    none = torch.zeros(0, dtype=torch.int64, device=cuda)
+    dy = torch.zeros(1, 1, device=cuda).expand(0, 8)
+    assert dy.shape == (0, 8) and dy.stride() == (0, 0)
+    grad = kernels.embedding_grad(none, dy, torch.ones(5, 8, device=cuda))
+    assert not grad.any()
