@@ -173,6 +173,11 @@ int64_t row_pitch(const Tensor& t, const char* what) {
   return t.size(0) > 1 ? t.stride(0) : t.size(1);
 }
 
+// A gradient of looked-up rows, of any shape, as one row per token.
+Tensor token_rows(const Tensor& dy, int64_t n, int64_t dim) {
+  return row_matrix(dy) ? dy : dy.reshape({n, dim}).contiguous();
+}
+
 void run_embedding(const Tensor& tokens, const Tensor& table, const Tensor& out, double scale, const Mask& m) {
   check_bound();
   check_devices({&tokens, &table, &out});
@@ -298,7 +303,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
       if (leaf != ctx->saved_data.end()) into = leaf->second.toTensor().grad();
       if (into.defined()) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "grad_in_place does not support create_graph");
-        const Tensor dy = row_matrix(dys[0]) ? dys[0] : dys[0].reshape({-1, table[1]}).contiguous();
+        const Tensor dy = token_rows(dys[0], saved[0].numel(), table[1]);
         run_grad(saved[0], dy, into, call.scale, call.padding, call.mask, true);
       } else {
         dw = table_grad(dys[0], saved[0], {table[0], table[1]}, static_cast<at::ScalarType>(table[2]), call);
@@ -314,7 +319,7 @@ struct TableGrad : torch::autograd::Function<TableGrad> {
     ctx->saved_data["call"] = call.save();
     ctx->saved_data["dy"] = static_cast<int64_t>(dy.scalar_type());
     ctx->save_for_backward({tokens, call.mask.state});
-    const Tensor rows = row_matrix(dy) ? dy : dy.reshape({-1, shape[1]}).contiguous();
+    const Tensor rows = token_rows(dy, tokens.numel(), shape[1]);
     Tensor dw = at::empty(shape, dy.options().dtype(dtype).memory_format(at::MemoryFormat::Contiguous));
     run_grad(tokens, rows, dw, call.scale, call.padding, call.mask, false);
     return dw;

@@ -100,3 +100,14 @@ def test_rows_of_empty_matrices_lie_anywhere(cuda):
     assert dy.shape == (0, 8) and dy.stride() == (0, 0)
     grad = kernels.embedding_grad(none, dy, torch.ones(5, 8, device=cuda))
     assert not grad.any()
+
+
+@pytest.mark.parametrize("tokens", [(), (3,), (2, 3), (1, 2, 3)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_backward_of_a_table_without_columns(cuda, tokens, in_place):
+    w = torch.empty(6, 0, device=cuda, requires_grad=True)
+    if in_place:
+        w.grad = torch.empty(6, 0, device=cuda)
+    y = nn.embedding(torch.zeros(tokens, dtype=torch.int64, device=cuda), w, grad_in_place=in_place)
+    y.sum().backward()
+    assert y.shape == (*tokens, 0) and w.grad.shape == (6, 0)
