@@ -226,6 +226,12 @@ void run_grad(const Tensor& tokens, const Tensor& dy, const Tensor& grad, double
                scratch.mutable_data_ptr(), bytes, stream_of(dev)));
 }
 
+// Graphs that saved the caller's buffer learn that it has been written.
+// (Tensors of inference mode have no counter.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- autograd --------------------------------------------------------------------
 // Scalars of a call, kept between forward and backward as one list.
 struct Call {
@@ -305,6 +311,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "grad_in_place does not support create_graph");
         const Tensor dy = token_rows(dys[0], saved[0].numel(), table[1]);
         run_grad(saved[0], dy, into, call.scale, call.padding, call.mask, true);
+        written(into);
       } else {
         dw = table_grad(dys[0], saved[0], {table[0], table[1]}, static_cast<at::ScalarType>(table[2]), call);
       }
@@ -413,6 +420,7 @@ PyObject* dfc_py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Mask m = mask_arg(a + 2);
   run_dropout(tensor_arg(a[0], "x"), optional_tensor(a[6], "residual"), tensor_arg(a[1], "out"), m);
+  written(THPVariable_Unpack(a[1]));
   Py_INCREF(a[1]);
   return a[1];
   END_HANDLE_TH_ERRORS
@@ -424,6 +432,7 @@ PyObject* dfc_py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Mask m = mask_arg(a + 4);
   run_embedding(tensor_arg(a[0], "tokens"), tensor_arg(a[1], "table"), tensor_arg(a[2], "out"), double_arg(a[3]), m);
+  written(THPVariable_Unpack(a[2]));
   Py_INCREF(a[2]);
   return a[2];
   END_HANDLE_TH_ERRORS
@@ -440,6 +449,7 @@ PyObject* dfc_py_embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (accumulate < 0) throw python_error();
   run_grad(tensor_arg(a[0], "tokens"), tensor_arg(a[1], "dy"), grad, double_arg(a[3]),
            padding_row(optional_int(a[4]), grad.size(0)), m, accumulate != 0);
+  written(grad);
   Py_INCREF(a[2]);
   return a[2];
   END_HANDLE_TH_ERRORS

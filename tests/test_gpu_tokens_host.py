@@ -111,3 +111,45 @@ def test_backward_of_a_table_without_columns(cuda, tokens, in_place):
     y = nn.embedding(torch.zeros(tokens, dtype=torch.int64, device=cuda), w, grad_in_place=in_place)
     y.sum().backward()
     assert y.shape == (*tokens, 0) and w.grad.shape == (6, 0)
+
+
+def test_autograd_sees_that_buffers_are_written(cuda):
+    """A buffer that a graph has saved and that a call then overwrites: its
+    backward raises, as after any in-place operation, instead of using the new
+    values."""
+    table = torch.randn(6, 8, device=cuda)
+    tok = torch.arange(4, device=cuda)
+    calls = {
+        "embedding": lambda b: kernels.embedding(tok, table, b),
+        "dropout": lambda b: kernels.dropout(table[:4], b, 0.5),
+        "dropout in place": lambda b: kernels.dropout(b, b, 0.5),
+        "grad": lambda b: kernels.embedding_grad(tok, table[:4], b),
+        "grad added": lambda b: kernels.embedding_grad(tok, table[:4], b, accumulate=True),
+    }
+    for name, write in calls.items():
+        buf = torch.randn(4, 8, device=cuda)
+        w = torch.ones(4, 8, device=cuda, requires_grad=True)
+        y, want = (buf * w).sum(), buf.clone()
+        y.backward(retain_graph=True)
+        assert torch.equal(w.grad, want)
+        before = buf._version
+        assert write(buf) is buf
+        assert buf._version == before + 1, name
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    w = table.clone().requires_grad_()
+    w.grad = torch.zeros_like(w)
+    v = torch.ones_like(w).requires_grad_()
+    y = (w.grad * v).sum()
+    nn.embedding(tok, w, grad_in_place=True).sum().backward()
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    assert not nn.dropout(table, 0.5)._version and not nn.embedding(tok, w)._version
+
+
+def test_buffers_of_inference_mode_are_written_as_before(cuda):
+    table = torch.randn(6, 8, device=cuda)
+    tok = torch.arange(4, device=cuda)
+    with torch.inference_mode():
+        out = kernels.embedding(tok, table, torch.empty(4, 8, device=cuda))
+    assert torch.equal(kernels.dropout(out, out, 0.0), table[:4])
