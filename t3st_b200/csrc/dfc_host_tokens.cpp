@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/Event.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -18,6 +19,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
@@ -278,6 +280,41 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
+// Autograd adds to a leaf's .grad on the stream of the leaf's accumulator, and
+// backward() puts its caller's stream behind that one.  Rows added in place are
+// added on the stream of the forward instead, which may be another one (where
+// the accumulator was made by an earlier use of the leaf): it waits for what the
+// accumulator's has done so far, and that one for the rows.
+class AccumulatorOrder {
+ public:
+  explicit AccumulatorOrder(const Tensor& leaf) : here_(c10::cuda::getCurrentCUDAStream(leaf.device().index())) {
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+    if (accumulator) there_ = accumulator->stream();
+    if (there_ && (there_->device_type() != c10::DeviceType::CUDA || *there_ == here_)) there_.reset();
+    if (!there_) return;
+    TORCH_CHECK(capturing(here_) == capturing(*there_),
+                "grad_in_place: this backward pass is captured, but the weight's gradient accumulator belongs to "
+                "a graph that was made outside the capture; delete that graph first");
+    order(*there_, here_);
+  }
+  void added() const {
+    if (there_) order(here_, *there_);
+  }
+
+ private:
+  static bool capturing(const c10::Stream& s) {
+    const c10::cuda::CUDAStreamGuard guard(s);
+    return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+  }
+  static void order(const c10::Stream& first, const c10::Stream& then) {
+    c10::Event e(c10::DeviceType::CUDA);
+    e.record(first);
+    e.block(then);
+  }
+  c10::Stream here_;
+  std::optional<c10::Stream> there_;  // the accumulator's, if another
+};
+
 // The lookup and the table's gradient are each other's gradient.
 Tensor table_grad(const Tensor& dy, const Tensor& tokens, at::IntArrayRef shape, at::ScalarType dtype,
                   const Call& call);
@@ -310,7 +347,9 @@ struct Embedding : torch::autograd::Function<Embedding> {
       if (into.defined()) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "grad_in_place does not support create_graph");
         const Tensor dy = token_rows(dys[0], saved[0].numel(), table[1]);
+        const AccumulatorOrder order(leaf->second.toTensor());
         run_grad(saved[0], dy, into, call.scale, call.padding, call.mask, true);
+        order.added();
         written(into);
       } else {
         dw = table_grad(dys[0], saved[0], {table[0], table[1]}, static_cast<at::ScalarType>(table[2]), call);

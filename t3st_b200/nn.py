@@ -93,8 +93,11 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
     ``ShardedDFCAdamW``, which owns it), backward adds the touched rows to it
     directly instead of returning a dense gradient to be added.  For leaf
     weights under ``backward()``; not for ``torch.autograd.grad``, and hooks on
-    the weight's gradient do not see it.  The buffer must have been zeroed on
-    the stream that ran this forward, or be ordered before it.
+    the weight's gradient do not see it.  The rows are added on the stream that
+    ran this forward.  They are ordered with gradients that reach the weight in
+    other ways, and what the caller of ``backward()`` launches next on its
+    stream sees them.  The buffer must have been zeroed on the stream that ran
+    this forward, or be ordered before it.
     """
     seed, state = _generator(seed)
     return _lib.host().nn_embedding(tokens, weight, scale, padding_idx, p, seed, offset, state,

@@ -153,3 +153,74 @@ def test_buffers_of_inference_mode_are_written_as_before(cuda):
     with torch.inference_mode():
         out = kernels.embedding(tok, table, torch.empty(4, 8, device=cuda))
     assert torch.equal(kernels.dropout(out, out, 0.0), table[:4])
+
+
+@pytest.mark.parametrize("caller", ["default", "forward", "third"])
+@pytest.mark.parametrize("tied", [False, True])
+def test_in_place_rows_are_ordered_behind_and_before_the_accumulator(cuda, caller, tied):
+    """The weight's accumulator was made on the default stream, the lookup runs
+    on another one, where its backward is held up: what follows backward() on
+    its caller's stream, and a dense gradient of the same weight (tied to a
+    second use), come after the rows."""
+    gen = torch.Generator().manual_seed(4)
+    tok = torch.randint(0, 40, (300,), generator=gen).cuda()
+    dy = torch.randint(-8, 9, (300, 64), generator=gen).float().cuda()
+    dense = torch.randint(-8, 9, (40, 64), generator=gen).float().cuda()
+    w = torch.randn(40, 64, generator=gen).cuda().requires_grad_()
+    want = torch.zeros_like(w).index_add_(0, tok, dy)  # whole numbers: exact in any order
+    if tied:
+        want = want + dense
+    main, side, third = torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()
+    w.grad = torch.zeros_like(w)
+    other = w * dense  # makes the accumulator
+    side.wait_stream(main)
+    with torch.cuda.stream(side):
+        out = nn.embedding(tok, w, grad_in_place=True)
+        out.register_hook(lambda g: torch.cuda._sleep(100_000_000))  # about 50 ms, in the backward
+        loss = (out * dy).sum()
+    main.wait_stream(side)
+    if tied:
+        loss = loss + other.sum()
+    stream = {"default": main, "forward": side, "third": third}[caller]
+    stream.wait_stream(main)
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            loss.backward(retain_graph=True)
+        got = w.grad.clone()
+    torch.cuda.synchronize()
+    assert torch.equal(got, 2 * want) and torch.equal(w.grad, 2 * want)
+
+
+def test_captured_in_place_backward_beside_an_eager_graph_is_refused(cuda):
+    """Ordering a capture behind an eager graph's stream is not possible: the
+    call raises, and the process goes on."""
+    code = """
+import torch
+from t3st_b200 import nn
+
+w = torch.randn(10, 8, device="cuda").requires_grad_()
+tok = torch.arange(5, device="cuda")
+w.grad = torch.zeros_like(w)
+eager = nn.embedding(tok, w, grad_in_place=True)  # alive: its accumulator is the default stream's
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+dy = torch.ones(5, 8, device="cuda")
+said = ""
+with torch.cuda.graph(graph):
+    try:
+        nn.embedding(tok, w, grad_in_place=True).backward(dy)
+    except RuntimeError as e:
+        said = str(e)
+assert "made outside the capture" in said, said
+del eager
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    nn.embedding(tok, w, grad_in_place=True).backward(dy)
+w.grad.zero_()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(w.grad[:5], dy) and not w.grad[5:].any()
+print("refused")
+"""
+    out = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "refused", out.stderr
