@@ -18,6 +18,8 @@ the same bits for the same inputs.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _lib
@@ -37,13 +39,28 @@ class CounterRng(torch.nn.Module):
     ``advance()`` draws new masks at each replay.  The state is a buffer:
     checkpoints carry it.  ``advance()`` between a forward and its backward
     makes that backward raise, as any in-place change of a saved tensor does.
+
+    ``rank``: ranks with data of their own (data parallel) each give their
+    number, or all drop the same elements; ranks that hold the same activations
+    (tensor parallel) give the same one.  It is not part of the state, so that
+    broadcast buffers and a checkpoint loaded on every rank leave the ranks
+    apart.  R ranks (rounded up to a power of two) share no mask for
+    2^32 / R steps.  ``state`` alone, given as a seed, is rank 0's.
     """
 
-    def __init__(self, seed: int = 0, device=None):
+    rank = base = 0  # counters pickled without a rank
+
+    def __init__(self, seed: int = 0, device=None, *, rank: int = 0):
         super().__init__()
         seed = int(seed) & 0xFFFFFFFFFFFFFFFF
+        rank = operator.index(rank)
+        if not 0 <= rank < 1 << 32:
+            raise ValueError("rank must be in [0, 2^32)")
         self.register_buffer("state", torch.tensor(
             [seed - (1 << 64) if seed >> 63 else seed, 0], dtype=torch.int64, device=device))
+        # added to every offset: the bits of the rank, reversed, so that few
+        # ranks lie far apart in the 64 bits
+        self.rank, self.base = rank, int(f"{rank:064b}"[::-1], 2)
         self._sites = 0
 
     def site(self) -> int:
@@ -58,13 +75,13 @@ class CounterRng(torch.nn.Module):
         self.state[1:].add_(_SITES)
 
 
-def _generator(seed):
-    """(seed, state) of a seed argument: an integer, a CounterRng or its tensor."""
+def _generator(seed, offset):
+    """(seed, offset, state) of a seed argument: an integer, a CounterRng or its tensor."""
     if isinstance(seed, CounterRng):
-        return 0, seed.state
+        return 0, operator.index(offset) + seed.base, seed.state
     if isinstance(seed, torch.Tensor):
-        return 0, seed
-    return seed, None
+        return 0, offset, seed
+    return seed, offset, None
 
 
 def dropout(x: torch.Tensor, p: float, *, seed=0, offset: int = 0,
@@ -74,7 +91,7 @@ def dropout(x: torch.Tensor, p: float, *, seed=0, offset: int = 0,
     (seed, offset, i) alone.  ``seed``: an int, a :class:`CounterRng` or a CUDA
     int64 tensor (seed, offset).  x: FP32, bf16 or fp16, any strides (the
     result is contiguous); residual: x's shape and dtype."""
-    seed, state = _generator(seed)
+    seed, offset, state = _generator(seed, offset)
     return _lib.host().nn_dropout(x, p, seed, offset, state, residual)
 
 
@@ -99,7 +116,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
     stream sees them.  The buffer must have been zeroed on the stream that ran
     this forward, or be ordered before it.
     """
-    seed, state = _generator(seed)
+    seed, offset, state = _generator(seed, offset)
     return _lib.host().nn_embedding(tokens, weight, scale, padding_idx, p, seed, offset, state,
                                     out_dtype, grad_in_place)
 

@@ -224,3 +224,12 @@ print("refused")
 """
     out = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip() == "refused", out.stderr
+
+
+def test_masks_of_a_rank(cuda):
+    x = torch.randn(1000, device=cuda)
+    for rank, base in ((0, 0), (1, 1 << 63), (3, 3 << 62), (6, 3 << 61)):
+        rng = nn.CounterRng(seed=5, rank=rank, device=cuda)
+        rng.advance()
+        want = nn.dropout(x, 0.3, seed=5, offset=base + (1 << 32) + 2)
+        assert torch.equal(nn.dropout(x, 0.3, seed=rng, offset=2), want)
