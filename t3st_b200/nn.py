@@ -48,7 +48,7 @@ class CounterRng(torch.nn.Module):
     2^32 / R steps.  ``state`` alone, given as a seed, is rank 0's.
     """
 
-    rank = base = 0  # counters pickled without a rank
+    rank = base = _spares = 0  # counters pickled without them
 
     def __init__(self, seed: int = 0, device=None, *, rank: int = 0):
         super().__init__()
@@ -65,10 +65,18 @@ class CounterRng(torch.nn.Module):
 
     def site(self) -> int:
         """A new site number."""
-        if self._sites >= _SITES:
+        if self._sites + self._spares >= _SITES:
             raise RuntimeError("too many dropout sites")
         self._sites += 1
         return self._sites - 1
+
+    def spare_site(self) -> int:
+        """A new site number from the other end, for a place that does not drop
+        yet: the numbers that site() gives do not depend on it."""
+        if self._sites + self._spares >= _SITES:
+            raise RuntimeError("too many dropout sites")
+        self._spares += 1
+        return _SITES - self._spares
 
     @torch.no_grad()
     def advance(self) -> None:
@@ -159,7 +167,7 @@ class Embedding(torch.nn.Module):
                 raise ValueError("padding_idx must be within the table")
             padding_idx %= num_embeddings
         self.padding_idx, self.scale, self.p, self.rng = padding_idx, float(scale), float(p), rng
-        self.site = rng.site() if p else 0
+        self.site = 0 if rng is None else rng.site() if p else rng.spare_site()
         self.out_dtype, self.grad_in_place = out_dtype, grad_in_place
         self.weight = torch.nn.Parameter(torch.empty(num_embeddings, embedding_dim, device=device,
                                                      dtype=dtype))
@@ -173,6 +181,8 @@ class Embedding(torch.nn.Module):
 
     def forward(self, tokens):
         p = self.p if self.training else 0.0
+        if p and self.rng is None:
+            raise ValueError("dropout needs a CounterRng")
         return embedding(tokens, self.weight, self.scale, padding_idx=self.padding_idx, p=p,
                          seed=self.rng if p else 0, offset=self.site, out_dtype=self.out_dtype,
                          grad_in_place=self.grad_in_place)
