@@ -405,7 +405,7 @@ struct SumArgs {
   uint32_t vocab, dim;
   float scale;
   int accumulate;
-  int wide_dy, wide_grad;  // rows on 32-byte boundaries
+  int wide_grad;  // rows on 32-byte boundaries
   Tokens tokens;         // SMALL: sorted by every CTA; the first one writes `keys` out for the join
   uint32_t* keys_out;
   float* partial;        // 2 rows a block: a run from before it, a run that goes on behind it
@@ -1278,7 +1278,6 @@ extern "C" int dfc_embedding_grad(const void* tokens, int32_t token_bytes, int64
   s.scale = drop ? static_cast<float>(static_cast<double>(scale) * (dropout->p < 1.0 ? 1.0 / (1.0 - dropout->p) : 0.0))
                  : scale;
   s.accumulate = accumulate != 0;
-  s.wide_dy = aligned(dy, 32) && dy_pitch % 8 == 0;
   s.wide_grad = aligned(grad, 32) && grad_pitch % 8 == 0;
   s.partial = reinterpret_cast<float*>(base + l.partial);
   s.partial_pitch = static_cast<uint32_t>(l.partial_pitch);
