@@ -18,6 +18,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -280,6 +281,16 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
+// This backward pass adds to the leaf's .grad (and does not hand the gradient
+// to a caller of torch.autograd.grad).
+bool accumulates(const Tensor& leaf) {
+  const auto* only = torch::autograd::get_current_graph_task_exec_info();
+  if (!only || only->empty()) return true;  // every leaf of the graph
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  const auto info = only->find(accumulator.get());
+  return info != only->end() && info->second.needed_;
+}
+
 // Autograd adds to a leaf's .grad on the stream of the leaf's accumulator, and
 // backward() puts its caller's stream behind that one.  Rows added in place are
 // added on the stream of the forward instead, which may be another one (where
@@ -343,7 +354,8 @@ struct Embedding : torch::autograd::Function<Embedding> {
     if (dys[0].defined() && ctx->needs_input_grad(0)) {
       const auto leaf = ctx->saved_data.find("leaf");
       Tensor into;
-      if (leaf != ctx->saved_data.end()) into = leaf->second.toTensor().grad();
+      if (leaf != ctx->saved_data.end() && accumulates(leaf->second.toTensor()))
+        into = leaf->second.toTensor().grad();
       if (into.defined()) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "grad_in_place does not support create_graph");
         const Tensor dy = token_rows(dys[0], saved[0].numel(), table[1]);

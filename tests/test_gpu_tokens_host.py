@@ -233,3 +233,32 @@ def test_masks_of_a_rank(cuda):
         rng.advance()
         want = nn.dropout(x, 0.3, seed=5, offset=base + (1 << 32) + 2)
         assert torch.equal(nn.dropout(x, 0.3, seed=rng, offset=2), want)
+
+
+def test_autograd_grad_of_an_in_place_weight(cuda):
+    """torch.autograd.grad asks for the gradient: it gets a dense one, and .grad
+    stays as it was.  backward(inputs=...) adds in place only to its inputs."""
+    tok = torch.randint(0, 20, (60,), generator=torch.Generator().manual_seed(5)).cuda()
+    w = torch.randn(20, 24, device=cuda).requires_grad_()
+    x = torch.randn(60, 24, device=cuda).requires_grad_()
+    dy = torch.randn(60, 24, device=cuda).requires_grad_()
+    kw = dict(padding_idx=3, p=0.3, seed=8, offset=9)
+    want = torch.autograd.grad(nn.embedding(tok, w, 2.0, **kw), w, dy)[0].detach()
+    w.grad = torch.ones_like(w)
+    y = nn.embedding(tok, w, 2.0, grad_in_place=True, **kw) + x
+    (dw,) = torch.autograd.grad(y, w, dy, retain_graph=True)
+    assert torch.equal(dw, want) and (w.grad == 1).all()
+    dw, dx = torch.autograd.grad(y, [w, x], dy, retain_graph=True)
+    assert torch.equal(dw, want) and torch.equal(dx, dy) and (w.grad == 1).all()
+    (dw,) = torch.autograd.grad(y, w, dy, create_graph=True)
+    (ddy,) = torch.autograd.grad(dw, dy, torch.ones_like(w))
+    ones = torch.ones_like(w)
+    ones[3] = 0
+    assert torch.equal(ddy, nn.embedding(tok, ones, 2.0, **kw))
+    y.backward(dy, inputs=[x], retain_graph=True)
+    assert (w.grad == 1).all()
+    grad = w.grad
+    y.backward(dy, inputs=[w], retain_graph=True)
+    assert w.grad is grad and torch.equal(grad, want + 1)
+    y.backward(dy)
+    assert w.grad is grad and torch.equal(grad, want + 1 + want)
