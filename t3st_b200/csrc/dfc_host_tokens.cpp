@@ -281,12 +281,14 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
-// This backward pass adds to the leaf's .grad (and does not hand the gradient
-// to a caller of torch.autograd.grad).
+// This backward pass adds to the leaf's .grad, does not hand the gradient to a
+// caller of torch.autograd.grad, and nothing looks at the gradient on its way.
+// (Hooks that run after the accumulation find it in .grad.)
 bool accumulates(const Tensor& leaf) {
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!accumulator || !accumulator->tensor_pre_hooks().empty() || !accumulator->pre_hooks().empty()) return false;
   const auto* only = torch::autograd::get_current_graph_task_exec_info();
   if (!only || only->empty()) return true;  // every leaf of the graph
-  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
   const auto info = only->find(accumulator.get());
   return info != only->end() && info->second.needed_;
 }

@@ -117,12 +117,13 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
     ``grad_in_place``: when ``weight`` already has a ``.grad`` (as under
     ``ShardedDFCAdamW``, which owns it), backward adds the touched rows to it
     directly instead of returning a dense gradient to be added.  For leaf
-    weights; ``torch.autograd.grad`` gets a dense gradient all the same.  Hooks
-    on the weight's gradient do not see it.  The rows are added on the stream that
-    ran this forward.  They are ordered with gradients that reach the weight in
-    other ways, and what the caller of ``backward()`` launches next on its
-    stream sees them.  The buffer must have been zeroed on the stream that ran
-    this forward, or be ordered before it.
+    weights; ``torch.autograd.grad`` and hooks on the weight's gradient get a
+    dense gradient all the same (hooks that run after its accumulation find the
+    rows in ``.grad``).  The rows are added on the stream that ran this forward.
+    They are ordered with gradients that reach the weight in other ways, and
+    what the caller of ``backward()`` launches next on its stream sees them.
+    The buffer must have been zeroed on the stream that ran this forward, or be
+    ordered before it.
     """
     seed, offset, state = _generator(seed, offset)
     return _lib.host().nn_embedding(tokens, weight, scale, padding_idx, p, seed, offset, state,

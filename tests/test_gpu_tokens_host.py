@@ -262,3 +262,56 @@ def test_autograd_grad_of_an_in_place_weight(cuda):
     assert w.grad is grad and torch.equal(grad, want + 1)
     y.backward(dy)
     assert w.grad is grad and torch.equal(grad, want + 1 + want)
+
+
+def test_hooks_see_an_in_place_weights_gradient(cuda):
+    """A hook on the weight's gradient, or on its accumulation, needs the dense
+    gradient: it gets it, with the result that a dense gradient gives."""
+    tok = torch.randint(0, 20, (60,), generator=torch.Generator().manual_seed(5)).cuda()
+    w = torch.randn(20, 24, device=cuda).requires_grad_()
+    dy = torch.randn(60, 24, device=cuda)
+    want = torch.autograd.grad(nn.embedding(tok, w, 2.0), w, dy)[0]
+
+    def backward():
+        w.grad = torch.ones_like(w)
+        nn.embedding(tok, w, 2.0, grad_in_place=True).backward(dy)
+        return w.grad
+
+    assert torch.equal(backward(), want + 1)
+    hook = w.register_hook(lambda g: g * 2)
+    assert torch.equal(backward(), want * 2 + 1)
+    hook.remove()
+    seen = []
+    hook = w.register_post_accumulate_grad_hook(lambda p: seen.append(p.grad.clone()))
+    assert torch.equal(backward(), want + 1) and len(seen) == 1 and torch.equal(seen[0], want + 1)
+    hook.remove()
+    accumulator = w.view_as(w).grad_fn.next_functions[0][0]
+    hook = accumulator.register_prehook(lambda g: (g[0] * 4,))
+    assert torch.equal(backward(), want * 4 + 1)
+    hook.remove()
+    assert torch.equal(backward(), want + 1) and len(seen) == 1
+
+
+def test_optimizer_in_the_backward_pass(cuda):
+    """Steps taken by hooks on accumulation happen with grad_in_place too."""
+    from t3st_b200 import DFCAdamW
+
+    tok = torch.randint(0, 50, (90,), generator=torch.Generator().manual_seed(5)).cuda()
+    finals = []
+    for in_place in (False, True):
+        torch.manual_seed(0)
+        emb = nn.Embedding(50, 16, grad_in_place=in_place, device=cuda)
+        opt = DFCAdamW(emb.parameters(), lr=1e-2)
+        emb.weight.grad = torch.zeros_like(emb.weight)
+
+        def step(p):
+            opt.step()
+            opt.zero_grad(set_to_none=False)
+
+        emb.weight.register_post_accumulate_grad_hook(step)
+        before = emb.weight.detach().clone()
+        for _ in range(3):
+            emb(tok).square().sum().backward()
+        assert not torch.equal(before, emb.weight)
+        finals.append(emb.weight.detach().clone())
+    assert torch.equal(*finals)
