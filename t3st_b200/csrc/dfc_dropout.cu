@@ -8,11 +8,13 @@
 // groups, in address order (the shape dfc_compress_ef measured best), all
 // loads issued before the first is used.
 //
-// Bounds (B200, 2^26 elements): FP32 with residual runs at the HBM floor of the
-// measured copy bandwidth (123 us), bf16 with residual too (60 us under ncu,
-// floor 61.5; 19 to 22 instructions an element).  bf16 without residual takes
-// about 52 us where HBM would need 41: there the ten rounds bound it, their
-// multiplications most of all.
+// Bounds (B200, 2^26 elements, p = 0.1, launch included; floors at the measured
+// copy bandwidth): FP32 with residual 123 us (floor 123), without 84 (82); bf16
+// with residual 65.5 (61.5; 24 instructions an element, 3.1 a cycle and SM),
+// without 57 (41; 21 instructions, 2.9 a cycle and SM).  The last is bound by the
+// issue of instructions: of the four a cycle that an SM can start three are
+// used, the ALU pipe (comparisons, selections, xors) is at 62% of its peak and
+// the pipe of the rounds' wide products at 44%.
 #include "dfc_philox.cuh"
 
 namespace dfc {
@@ -20,7 +22,8 @@ namespace {
 
 constexpr int kThreads = 256;
 // Groups per thread: two for 16-bit types, one for FP32 (32 bytes of each
-// operand in flight per thread either way), and registers for 6 CTAs per SM.
+// operand in flight per thread either way), and registers for 6 CTAs per SM (40;
+// the 16-bit forms with residual and dropout spill 24 bytes a thread there).
 // Of 1, 2 and 4 groups at 3 to 6 CTAs, 2^26 elements with residual, launch
 // included: bf16 65.5 us (1 group 73.7; 4 groups 65.5 at 3 CTAs, but 8.2 us
 // instead of 6.2 for 2^16 elements), FP32 122.9 us (2 groups 124.9, 4 groups 132).
@@ -91,6 +94,9 @@ __global__ void __launch_bounds__(kThreads, 6)
   }
 }
 
+// Any alignment: element accesses, 16 or 32 bytes apart between lanes.  2^26
+// elements off 16-byte boundaries: bf16 174 us, with residual 180, FP32 283 and
+// 297; loads in flight bound it (1.4 instructions a cycle and SM).
 template <typename T, bool RES, bool DROP>
 __global__ void __launch_bounds__(kThreads)
     dropout_any_kernel(const T* x, const T* res, T* y, int64_t n, DropArgs a) {
